@@ -22,7 +22,7 @@ CSRC = os.path.join(ROOT, "csrc")
 HEADER = os.path.join(REPO, "include", "crog_hip.h")
 LIB_PATH = os.environ.get("CROG_LIB") or os.path.join(ROOT, "libcrog_hip.so")
 BUILD_DIR = os.path.join(ROOT, "csrc", "build")
-SOURCES = ["api.hip", "gemm.hip", "gemm_pp.hip", "gemm_ppt.hip", "conv_sw.hip", "wgrad_sw.hip", "gemm_skinny.hip", "norm.hip", "eltwise.hip", "head.hip", "conv_aux.hip", "attn.hip", "ssg.hip", "preprocess.hip", "replay.hip", "comm.hip"]
+SOURCES = ["api.hip", "gemm.hip", "gemm_pp.hip", "gemm_ppt.hip", "conv_sw.hip", "wgrad_sw.hip", "gemm_skinny.hip", "norm.hip", "eltwise.hip", "head.hip", "conv_aux.hip", "attn.hip", "packed_attn.hip", "rotary.hip", "gated_norm.hip", "ssg.hip", "preprocess.hip", "replay.hip", "comm.hip"]
 # NO_PACKED_F32: the device code is built WITHOUT the packed-fp32 VALU instructions (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32: what the
 # SLP vectoriser makes of adjacent scalar fp32 operations - 19 880 of them in 236 kernels under plain -O3).  Round 5 found their results wrong
 # in lanes 48-63 of a wave when an MFMA kernel of ANOTHER stream shares the SIMD: the bilinear x2 backward beside a weight-gradient GEMM

@@ -20,6 +20,7 @@ from typing import List, Optional, Tuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import kernels as K
 from .runtime import RT, ParamStore, slab_scratch
@@ -1239,6 +1240,187 @@ def mha(xq, xk, xv, wq: WRef, wk: WRef, wv: WRef, bq, bk, bv, wo: WRef, bo, *, B
     params = params + [None] * (8 - len(params))
     kvbuf, joint = kv if kv is not None else (None, None)
     return MhaFn.apply(xq, xk, xv, res, kvbuf, *params, wq, wk, wv, bq, bk, bv, wo, bo, B, heads, causal, kpm, float(p_drop), res_slot, joint)
+
+
+# ------------------------------------------------------------------------------------------------
+# a transformer block on packed rows: attention, rotary positions, the gated residual between two norms
+# ------------------------------------------------------------------------------------------------
+class PackedAttentionFn(Function):
+    """o = softmax(scale q k^T) v within each sequence of a PackedRows plan (the packed form of the attention inside MhaFn: clip.py:246-260,
+    layers.py:291-296,329-332), any head dim up to 128, grouped key heads."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, rows, scale):
+        ctx.set_materialize_grads(False)
+        ctx.shapes = (q.shape, k.shape, v.shape)
+        empty = rows.rows_q == 0 or rows.rows_k == 0
+        o = (torch.zeros if empty else torch.empty)(q.shape, device=q.device, dtype=q.dtype)
+        lse = None
+        if not empty:
+            q, k, v = K.heads16(q), K.heads16(k), K.heads16(v)
+            if any(ctx.needs_input_grad):
+                lse = torch.empty(rows.rows_q * q.shape[1], device=q.device, dtype=torch.float32)
+            K.packed_attn_fwd(q, k, v, o, lse, rows, scale)
+            if q.shape[0] > rows.rows_q:
+                o[rows.rows_q:].zero_()
+        ctx.cfg = (rows, scale)
+        ctx.save_for_backward(*((q, k, v, o, lse) if lse is not None else ()))
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        if do is None:
+            return (None,) * 5
+        rows, scale = ctx.cfg
+        if not ctx.saved_tensors:
+            return tuple(torch.zeros(s, device=do.device, dtype=do.dtype) for s in ctx.shapes) + (None, None)
+        q, k, v, o, lse = ctx.saved_tensors
+        do = K.heads16(do)
+        dq, dk, dv = (torch.empty(s, device=q.device, dtype=q.dtype) for s in ctx.shapes)
+        K.packed_attn_bwd(q, k, v, o, do, lse, torch.empty_like(lse), dq, dk, dv, rows, scale)
+        for t, n in ((dq, rows.rows_q), (dk, rows.rows_k), (dv, rows.rows_k)):
+            if t.shape[0] > n:
+                t[n:].zero_()
+        return dq, dk, dv, None, None
+
+
+def packed_attention(q, k, v, rows, scale=None):
+    """q [rows, heads, dim], k and v [key rows, heads / group, dim], float32 or bfloat16, in the order of `rows` (packed.PackedRows: lengths,
+    group, causal); any strides with adjacent columns (others are copied).  -> [rows, heads, dim].  scale: dim ** -0.5 by default.  dim is a
+    multiple of 8 up to 128 (float32: of 4).  Rows behind the last sequence give zeros and get zero gradients, whatever they hold.  The same
+    inputs give the same bits (no atomics).  A key or value that is not finite may reach every query of its own sequence, and no other."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise ValueError(f"packed_attention: {name} must be [rows, heads, dim], got {tuple(t.shape)}")
+    K.dcode(q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"packed_attention: q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.shape != v.shape or q.shape[2] != k.shape[2] or q.shape[1] != k.shape[1] * rows.group or k.shape[1] < 1:
+        raise ValueError(f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit a group of {rows.group} query heads per key head")
+    dim, vec = q.shape[2], 16 // q.element_size()
+    if not 0 < dim <= 128 or dim % vec:
+        raise ValueError(f"packed_attention: the head dimension must be a multiple of {vec} up to 128 for {q.dtype}, got {dim}")
+    if q.shape[0] < rows.rows_q or k.shape[0] < rows.rows_k:
+        raise ValueError(f"packed_attention: the plan has {rows.rows_q} query and {rows.rows_k} key rows, the tensors {q.shape[0]} and {k.shape[0]}")
+    if scale is not None and not math.isfinite(scale):
+        raise ValueError("packed_attention: scale must be finite")
+    K.same_device(q, k, v, rows._table)
+    return PackedAttentionFn.apply(q, k, v, rows, float(dim ** -0.5 if scale is None else scale))
+
+
+class RotaryFn(Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, axes):
+        ctx.set_materialize_grads(False)
+        ctx.axes = axes
+        ctx.save_for_backward(positions)
+        return RotaryFn._turn(q, k, positions, axes, False)
+
+    @staticmethod
+    def _turn(q, k, positions, axes, inverse):
+        q, k = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (q, k))
+        qo, ko = (None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+        if q is not None or k is not None:
+            K.rotary(q, k, qo, ko, positions, axes, inverse=inverse)
+        return qo, ko
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        positions, = ctx.saved_tensors
+        dq, dk = RotaryFn._turn(dq, dk, positions, ctx.axes, True)
+        return dq, dk, None, None
+
+
+def rotary(q, k, positions, axes):
+    """Turns q [rows, heads, dim] and k [rows, key heads, dim] (k may be None) by their rows' positions, an int32 / int64 tensor [rows, axes]
+    ([rows] for one axis), as `axes` (packed.RotaryAxes) says; -> (q', k').  Columns behind the plan's pairs are copied."""
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        raise ValueError(f"rotary: q and k must be [rows, heads, dim] with the same rows and dim, got {tuple(q.shape)}, {None if k is None else tuple(k.shape)}")
+    K.dcode(q)
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError(f"rotary: q and k must have one dtype, got {q.dtype} and {k.dtype}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"rotary: positions must be int32 or int64, got {positions.dtype}")
+    if positions.dim() == 1 and axes.axes == 1:
+        positions = positions[:, None]
+    if positions.shape != (q.shape[0], axes.axes):
+        raise ValueError(f"rotary: positions must be [{q.shape[0]}, {axes.axes}], got {tuple(positions.shape)}")
+    if 2 * axes.pairs > q.shape[2]:
+        raise ValueError(f"rotary: {axes.pairs} pairs do not fit heads of {q.shape[2]}")
+    K.same_device(q, k, positions, axes._table)
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    return RotaryFn.apply(q, k, positions, axes)
+
+
+class GatedNormFn(Function):
+    @staticmethod
+    def forward(ctx, x, y, gate, post, pre, alpha, eps, rms, *params):
+        ctx.set_materialize_grads(False)
+        u = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if pre is not None else None
+        stats = torch.empty(x.numel() // x.shape[-1], 4, device=x.device, dtype=torch.float32) if any(ctx.needs_input_grad) else None
+        masters = [None if w is None else tuple(r.master() if r is not None else None for r in w) for w in (post, pre)]
+        K.gated_norm_fwd(x, y, gate.master() if gate is not None else None, *masters, rms, alpha, eps, u, h, stats)
+        ctx.cfg = (gate, post, pre, alpha, rms)
+        ctx.save_for_backward(x, y, stats)
+        return u, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, du, dh):
+        gate, post, pre, alpha, rms = ctx.cfg
+        x, y, stats = ctx.saved_tensors
+        none = (None,) * (len(ctx.needs_input_grad) - 2)
+        if du is None and dh is None:
+            return (None, None) + none
+        du, dh = (K.as_mat(t) if t is not None else None for t in (du, dh))
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
+        dy = torch.empty(x.shape, device=x.device, dtype=x.dtype) if ctx.needs_input_grad[1] else None
+
+        def grad(r):
+            return r.grad() if r is not None and r.param.requires_grad else None
+        masters = [None if w is None else tuple(r.master() if r is not None else None for r in w) for w in (post, pre)]
+        post, pre = post or (None, None), pre or (None, None)
+        K.gated_norm_bwd(x, y, du, dh, gate.master() if gate is not None else None, *masters, rms, alpha, stats, dx, dy, grad(gate),
+                         [grad(r) for r in post], [grad(r) for r in pre])
+        for r in (gate, *post, *pre):
+            if grad(r) is not None:
+                r.done()
+        return (dx, dy) + none
+
+
+def gated_norm(x, y, *, post=None, gate: Optional[WRef] = None, pre=None, res_scale=1.0, eps=1e-5, rms=False):
+    """The residual between two blocks in one launch: z = norm(y) with `post` (y itself without it), u = res_scale * x + gate * z, and
+    h = norm(u) with `pre`; -> (u, h), h None without `pre`.  post / pre: (weight WRef, bias WRef or None); gate: WRef of one factor per column
+    (1 without it).  rms: root-mean-square norms (no biases) instead of LayerNorm.  x, y: row matrices [..., C] of one shape and dtype, C up to
+    8192; the second norm reads the float32 sum, u and h are rounded once.  The weights' gradients are added into the flat store in a fixed
+    order (same bits every time)."""
+    K.dcode(x)
+    if x.shape != y.shape or x.dtype != y.dtype or x.dim() < 1:
+        raise ValueError(f"gated_norm: x and y must have one shape and dtype, got {tuple(x.shape)} {x.dtype} and {tuple(y.shape)} {y.dtype}")
+    C = x.shape[-1]
+    if not 0 < C <= 8192:
+        raise ValueError(f"gated_norm: rows of 1 to 8192 columns, got {C}")
+    refs = [gate]
+    for name, w in (("post", post), ("pre", pre)):
+        if w is None:
+            continue
+        if len(w) != 2:
+            raise ValueError(f"gated_norm: {name} must be (weight, bias or None)")
+        if rms and w[1] is not None:
+            raise ValueError(f"gated_norm: a root-mean-square norm has no bias ({name})")
+        refs += list(w)
+    refs = [r for r in refs if r is not None]
+    for r in refs:
+        if r.rows * r.cols != C:
+            raise ValueError(f"gated_norm: a weight of {r.rows * r.cols} values for rows of {C} columns")
+    if not eps >= 0 or not math.isfinite(res_scale):
+        raise ValueError("gated_norm: eps must not be negative and res_scale must be finite")
+    K.same_device(x, y, *[r.P for r in refs])
+    return GatedNormFn.apply(K.as_mat(x), K.as_mat(y), gate, post, pre, float(res_scale), float(eps), bool(rms), *[r.param for r in refs])
 
 
 # ------------------------------------------------------------------------------------------------

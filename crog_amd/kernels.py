@@ -739,3 +739,87 @@ def ssg_match(anchors: torch.Tensor, gt: torch.Tensor, ng: torch.Tensor, pos_thr
     check(lib().crog_ssg_match(ptr(anchors), A, ptr(gt), ptr(ng), B, Gmax, float(pos_thr), float(neg_thr), ptr(claim), ptr(offsets), ptr(labels),
                                ptr(mbox), ptr(midx), stream()), "ssg_match")
     return offsets, labels, mbox, midx
+
+
+# --------------------------------------------------------------------------------------------
+# a transformer block on packed rows (crog_amd.packed holds the plans, crog_amd.functional the autograd forms)
+# --------------------------------------------------------------------------------------------
+def same_device(*ts):
+    """The kernels are launched on the current device's current stream: every tensor has to live there."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("crog_amd kernels need GPU tensors (there is no CPU path)")
+        if dev is None:
+            dev = torch.cuda.current_device()
+        if t.device.index != dev:
+            raise RuntimeError(f"a tensor lives on {t.device}, the current device is cuda:{dev}")
+
+
+def heads16(t: torch.Tensor) -> torch.Tensor:
+    """`t` [rows, heads, dim] if every head starts on a 16-byte boundary and its columns are adjacent, else a contiguous copy."""
+    vec = 16 // t.element_size()
+    if t.stride(2) == 1 and t.stride(0) % vec == 0 and t.stride(1) % vec == 0 and t.data_ptr() % 16 == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def packed_attn_fwd(q, k, v, o, lse, rows, scale):
+    """q [>= rows.rows_q, kv_heads * group, dim], k, v [>= rows.rows_k, kv_heads, dim]; rows: packed.PackedRows."""
+    kv, dim = k.shape[1], k.shape[2]
+    splits, piece = rows.splits(kv)
+    ws = torch.empty(splits * kv * rows.rows_q * rows.group * (dim + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
+    check(lib().crog_packed_attn_fwd(dcode(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                     v.stride(1), o.data_ptr(), o.stride(0), o.stride(1), ptr(lse), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr,
+                                     rows.n_row_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, splits, piece,
+                                     ptr(ws), stream()), "packed_attn_fwd")
+
+
+def packed_attn_bwd(q, k, v, o, do, lse, D, dq, dk, dv, rows, scale):
+    kv, dim = k.shape[1], k.shape[2]
+    check(lib().crog_packed_attn_bwd(dcode(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                                     v.stride(1), o.data_ptr(), o.stride(0), o.stride(1), do.data_ptr(), do.stride(0), do.stride(1), ptr(lse), ptr(D),
+                                     dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1), dv.data_ptr(), dv.stride(0),
+                                     dv.stride(1), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr, rows.n_row_tiles, rows.key_tiles_ptr,
+                                     rows.n_key_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, stream()),
+          "packed_attn_bwd")
+
+
+def rotary(q, k, q_out, k_out, positions, axes, inverse=False):
+    """q / k (either may be None): [rows, heads, dim] with adjacent columns; positions [rows, axes]; axes: packed.RotaryAxes."""
+    t = q if q is not None else k
+
+    def three(x):
+        return (None, 0, 0) if x is None else (x.data_ptr(), x.stride(0), x.stride(1))
+    check(lib().crog_rotary(dcode(t), *three(q), *three(k), *three(q_out), *three(k_out), positions.data_ptr(), positions.stride(0),
+                            positions.element_size(), axes.revs_ptr, axes.axis_ptr, t.shape[0], 0 if q is None else q.shape[1],
+                            0 if k is None else k.shape[1], t.shape[2], axes.pairs, axes.axes, axes.interleaved, int(inverse), stream()), "rotary")
+
+
+def gated_norm_fwd(x, y, gate, post, pre, rms, alpha, eps, u, h, stats):
+    """post / pre: None or (weight or None, bias or None), fp32 [C]; h None without a pre norm."""
+    M, C, ldx = mat(x)
+    pw, pb = post if post is not None else (None, None)
+    nw, nb = pre if pre is not None else (None, None)
+    check(lib().crog_gated_norm_fwd(dcode(x), x.data_ptr(), ldx, y.data_ptr(), mat(y)[2], ptr(gate), ptr(pw), ptr(pb), ptr(nw), ptr(nb),
+                                    int(post is not None), int(pre is not None), int(rms), float(alpha), float(eps), M, C, u.data_ptr(), mat(u)[2],
+                                    ptr(h), mat(h)[2] if h is not None else 0, ptr(stats), stream()), "gated_norm_fwd")
+
+
+def gated_norm_bwd(x, y, du, dh, gate, post, pre, rms, alpha, stats, dx, dy, dgate, dpost, dpre):
+    """dpost / dpre: (weight gradient or None, bias gradient or None), added onto."""
+    M, C, ldx = mat(x)
+    pw, pb = post if post is not None else (None, None)
+    sums = [dgate, *dpost, *dpre]
+    slab = None
+    if any(t is not None for t in sums):
+        slab = torch.empty(lib().crog_gated_norm_slab_floats(M, C), device=x.device, dtype=torch.float32)
+
+    def two(t):
+        return (None, 0) if t is None else (t.data_ptr(), mat(t)[2])
+    check(lib().crog_gated_norm_bwd(dcode(x), x.data_ptr(), ldx, y.data_ptr(), mat(y)[2], *two(du), *two(dh), ptr(gate), ptr(pw), ptr(pb),
+                                    ptr(pre[0]) if pre is not None else None, int(post is not None), int(pre is not None), int(rms), float(alpha), M, C,
+                                    ptr(stats), *two(dx), *two(dy), ptr(slab), *[ptr(t) for t in sums], stream()), "gated_norm_bwd")

@@ -606,6 +606,53 @@ int crog_preprocess_u8(const uint8_t* img, const uint8_t* masks, int B, int H, i
                        const int16_t* tab_cubic, const int16_t* tab_linear, int S, const float* mean, const float* stdv,
                        const int* border, float* out_img, float* out_masks, crog_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * A transformer block on PACKED rows: sequences of different lengths one behind the other, no padding between them (crog_amd/packed.py builds
+ * the tables; the padded forms are crog_flash_attn_*, crog_ln_* and the positional tables of crog_embedding_fwd / crog_add_rows).
+ *
+ * Attention.  Element (row, head, d) of X lives at X + row * ldx + head * hsx + d, all of them multiples of 16 bytes; head_dim: multiples of 8
+ * (bf16) or 4 (fp32) up to 128; head kv * group + g of Q reads head kv of K / V.  Sequence s owns query rows cu_q[s] .. cu_q[s + 1] - 1 and key
+ * rows cu_k[s] .. (device int32 tables of seqs + 1 entries, not decreasing, at most rows_q / rows_k).  causal: query i of Lq sees keys
+ * j <= i + Lk - Lq (the ends aligned; a query that sees none gives zeros).  tiles: device int32 pairs (sequence, tile): blocks of 128 of the
+ * sequence's Lq * group rows (forward, dQ: row_tiles) or of 128 keys (key_tiles), each exactly once, in the order in which they should start.
+ * lse (may be NULL in the forward) and D: [kv_heads][rows_q * group] floats, base-2 logarithms, the forward's for the backward.
+ * splits > 1: the keys of a row are walked in `splits` pieces of split_keys (a multiple of 64; splits * split_keys >= the longest key
+ * sequence) that meet in a second launch; partial: splits * kv_heads * rows_q * group * (head_dim + 2) floats.
+ * Rows outside every sequence are not read and not written.  Non-finite values of a key or value row may reach every query row of its own
+ * sequence (also through a probability of zero), never another sequence. */
+int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64_t hsq, const void* K, int64_t ldk, int64_t hsk,
+                         const void* V, int64_t ldv, int64_t hsv, void* O, int64_t ldo, int64_t hso, float* lse, const int* cu_q,
+                         const int* cu_k, const int* tiles, int n_tiles, int seqs, int rows_q, int rows_k, int kv_heads, int group,
+                         int head_dim, float scale, int causal, int splits, int split_keys, float* partial, crog_stream_t stream);
+int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64_t hsq, const void* K, int64_t ldk, int64_t hsk,
+                         const void* V, int64_t ldv, int64_t hsv, const void* O, int64_t ldo, int64_t hso, const void* dO,
+                         int64_t lddo, int64_t hsdo, const float* lse, float* D, void* dQ, int64_t lddq, int64_t hsdq, void* dK,
+                         int64_t lddk, int64_t hsdk, void* dV, int64_t lddv, int64_t hsdv, const int* cu_q, const int* cu_k,
+                         const int* row_tiles, int n_row_tiles, const int* key_tiles, int n_key_tiles, int seqs, int rows_q,
+                         int rows_k, int kv_heads, int group, int head_dim, float scale, int causal, crog_stream_t stream);
+/* Rotary positions: the first 2 * pairs (at most 256) columns of every head of Q (heads_q) and K (heads_k, may be 0) are pairs - column i with
+ * column pairs + i, or, interleaved, 2 i with 2 i + 1 - that turn by positions[row * ldpos + axis[i]] * revs[i] revolutions (inverse: back);
+ * the other columns are copied.  positions: int32 or int64 (pos_bytes 4 / 8); revs: `pairs` doubles, axis: `pairs` ints below `axes`, on the
+ * device.  In place (Qout = Q with equal strides) is allowed. */
+int crog_rotary(int dtype, const void* Q, int64_t ldq, int64_t hsq, const void* K, int64_t ldk, int64_t hsk, void* Qout, int64_t ldqo,
+                int64_t hsqo, void* Kout, int64_t ldko, int64_t hsko, const void* positions, int64_t ldpos, int pos_bytes,
+                const void* revs, const int* axis, int rows, int heads_q, int heads_k, int head_dim, int pairs, int axes,
+                int interleaved, int inverse, crog_stream_t stream);
+/* The residual between two blocks: z = N(y) * post_w + post_b (has_post; else z = y), u = alpha * x + gate * z, h = N(u) * pre_w + pre_b
+ * (has_pre); N = LayerNorm's, or with rms the root-mean-square norm.  Weights fp32 [cols], NULL = 1 (post_w, pre_w, gate) or 0 (post_b,
+ * pre_b); cols <= 8192.  The second norm reads the fp32 sum.  stats: NULL or [rows][4] floats for the backward.
+ * Backward: du, dh may be NULL (no gradient); dx, dy may be NULL (not wanted); the weights' gradients are ADDED onto what their buffers hold
+ * (NULL = not wanted), through slab, crog_gated_norm_slab_floats(rows, cols) floats of scratch, in a fixed order. */
+int crog_gated_norm_slab_floats(int rows, int cols);
+int crog_gated_norm_fwd(int dtype, const void* x, int64_t ldx, const void* y, int64_t ldy, const float* gate, const float* post_w,
+                        const float* post_b, const float* pre_w, const float* pre_b, int has_post, int has_pre, int rms, float alpha,
+                        float eps, int rows, int cols, void* u, int64_t ldu, void* h, int64_t ldh, float* stats, crog_stream_t stream);
+int crog_gated_norm_bwd(int dtype, const void* x, int64_t ldx, const void* y, int64_t ldy, const void* du, int64_t lddu,
+                        const void* dh, int64_t lddh, const float* gate, const float* post_w, const float* post_b, const float* pre_w,
+                        int has_post, int has_pre, int rms, float alpha, int rows, int cols, const float* stats, void* dx, int64_t lddx,
+                        void* dy, int64_t lddy, float* slab, float* dgate, float* dpost_w, float* dpost_b, float* dpre_w,
+                        float* dpre_b, crog_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
