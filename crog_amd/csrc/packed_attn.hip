@@ -11,23 +11,24 @@
 // products; its k index is the lane's half, so the registers are that operand as they stand.
 // One LDS image serves both ways of reading a tile - rows (16 bytes a lane, lane = row) and columns (ds_read_b64_tr_b16, four rows x 64 bytes a
 // half wave): the 16-byte slot of a row is XORed with the row's low bits, the lowest two moved to the slot's high bits.
-#include "common.h"
+#include "gemm_dma.h"
 
 namespace {
 
-constexpr int NT = 256;      // 4 waves, 32 rows (forward, dQ) or 32 keys (dK / dV) each
-constexpr int BR = 128;      // rows (keys) of a block
+constexpr int NT = 256;      // 4 waves
+constexpr int BR = 128;      // rows of a block (forward, dQ)
+constexpr int BK = 64;       // keys of a block (dK / dV)
 
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
 struct PackedArgs {
   const void *Q, *K, *V, *O, *dO;
   void *Out, *dQ, *dK, *dV;
-  float *lse, *D;      // [kv_heads][rows_q * group], lse in log2 units (-inf: no key)
+  float *lse, *D;      // [heads][rows_q], lse in log2 units (-inf: no key)
   float *part_o, *part_ml;
   long ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso, lddo, hsdo, lddq, hsdq, lddk, hsdk, lddv, hsdv;
   const int *cu_q, *cu_k, *tiles;
-  int seqs, rows_q, rows_k, kv_heads, group, dim, causal, split_keys;
+  int seqs, rows_q, rows_k, kv_heads, group, dim, causal, split_keys, piece, parts;
   float scale;
 };
 
@@ -44,13 +45,40 @@ __device__ inline Seq seq_of(const PackedArgs& a, int s) {
 }
 
 // ---- LDS tiles of rows of DP elements ----------------------------------------------------------------------------------------
+// gemm_dma.h's request with a scalar offset besides the lane's (both below 2^31: their sum is out of range exactly where the lane's is DMA_OOB)
+__device__ __attribute__((always_inline)) inline void dma_piece_at(const void* base, char* dst, unsigned off, unsigned soff) {
+  typedef __attribute__((address_space(3))) char lds_char;
+  const unsigned long long b = (unsigned long long)base;
+  dma_i32x4 r;
+  r.x = __builtin_amdgcn_readfirstlane((int)(unsigned)b);
+  r.y = __builtin_amdgcn_readfirstlane((int)((unsigned)(b >> 32) & 0xffffu));
+  r.z = 0x7fffffff;
+  r.w = 0x00020000;
+  const unsigned m0v = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)(lds_char*)dst);
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m0v), "v"(off), "s"(r), "s"(soff) : "memory", "m0");
+}
+
+__device__ inline void opaque(int& x) { asm volatile("" : "+v"(x)); }      // keeps what is computed from x inside the loop it stands in
+
 template <typename T, int DP> struct Tile {
   static constexpr int VEC = Elem<T>::VEC, CPR = DP / VEC;      // 16-byte chunks per row
   static constexpr int NS = CPR / 2;                            // 16-byte operand steps of a lane (its half takes every other chunk)
   static constexpr int NC = DP / 32;                            // 32-column blocks
-  __device__ static inline int off(int row, int chunk) {
-    const int f = CPR == 8 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
-    return row * DP + ((chunk ^ f) * VEC);
+  __device__ static constexpr int slot(int row) { return CPR == 8 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3)); }
+  static constexpr int RB = DP * (int)sizeof(T);      // bytes of a row
+  // Byte offsets of a lane in a tile.  Its other operands of the tile differ from these by XORs with constants and by whole rows (an instruction's
+  // immediate), so a kernel keeps one register of each kind and XORs as it reads; all of them kept in registers made the backward kernels spill.
+  // rows: row `ln`, 16-byte step 0.  (step ks: ^ 32 ks)
+  __device__ static inline int rows_at(int lane) { return (lane & 31) * RB + (((lane >> 5) ^ slot(lane & 31)) << 4); }
+  // columns: bf16, 4 rows x 4 columns of the transposed read (column block c: ^ 64 c, the rows 8 further down: ^ 32); float, one column
+  __device__ static inline int cols_at(int lane) {
+    const int h = lane >> 5, ln = lane & 31;
+    if constexpr (sizeof(T) == 2) {
+      const int q = (lane & 15) >> 2, pp = lane & 3, row = 4 * h + q;
+      return row * RB + (((2 * ((lane >> 4) & 1) + (pp >> 1)) ^ slot(row)) << 4) + (pp & 1) * 8;
+    } else {
+      return 4 * h * RB + (((ln >> 2) ^ h) << 4) + (ln & 3) * 4;
+    }
   }
 };
 
@@ -58,13 +86,13 @@ __device__ inline int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 
 constexpr float LOG2E = 1.4426950408889634f;
 __device__ inline float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// acc (32 rows of the tile x 32 columns = lanes) += tile rows . frag (the lane's row of the other operand)
+// acc (32 rows of the tile x 32 columns = lanes) += tile rows . frag (the lane's row of the other operand).  at: rows_at + the buffer's offset
 template <typename T, int DP>
-__device__ inline void mma_rows(f32x16& acc, const T* tile, int row, int h, const Vec16<T>* frag) {
+__device__ inline void mma_rows(f32x16& acc, const T* tile, int at, int tile_row, const Vec16<T>* frag) {
   using L = Tile<T, DP>;
 #pragma unroll
   for (int ks = 0; ks < L::NS; ks++) {
-    const Vec16<T> a = ldg16(tile + L::off(row, 2 * ks + h));
+    const Vec16<T> a = ldg16((const T*)((const char*)tile + (at ^ (ks << 5)) + tile_row * L::RB));
     if constexpr (sizeof(T) == 2) {
       acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, frag[ks]), acc, 0, 0, 0);
     } else {
@@ -74,13 +102,11 @@ __device__ inline void mma_rows(f32x16& acc, const T* tile, int row, int h, cons
   }
 }
 
-// out[c] (columns 32 c .. 32 c + 31 of the tile x lanes) += tile^T . p, p = 32 tile rows (registers, acc_row order) x lanes
+// out[c] (columns 32 c .. 32 c + 31 of the tile x lanes) += tile^T . p, p = 32 tile rows (registers, acc_row order) x lanes.  at: cols_at + ...
 template <typename T, int DP>
-__device__ inline void mma_cols(f32x16* out, const T* tile, const f32x16& p, int lane) {
+__device__ inline void mma_cols(f32x16* out, const T* tile, int at, int tile_row, const f32x16& p) {
   using L = Tile<T, DP>;
-  const int h = lane >> 5;
   if constexpr (sizeof(T) == 2) {
-    const int i = lane & 15, q = i >> 2, pp = i & 3;
 #pragma unroll
     for (int t = 0; t < 2; t++) {
       bf16x8 b;      // (the probabilities are rounded to the operand type of the matrix unit: half a bf16 step each, as the inputs are)
@@ -88,20 +114,20 @@ __device__ inline void mma_cols(f32x16* out, const T* tile, const f32x16& p, int
       for (int j = 0; j < 8; j++) b[j] = (bf16)p[8 * t + j];
 #pragma unroll
       for (int c = 0; c < L::NC; c++) {
-        const int col = c * 32 + 16 * ((lane >> 4) & 1) + 4 * pp, chunk = col >> 3, inb = col & 7;
-        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + L::off(16 * t + 4 * h + q, chunk) + inb));
-        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(tile + L::off(16 * t + 8 + 4 * h + q, chunk) + inb));
+        const char* base = (const char*)tile + (tile_row + 16 * t) * L::RB;
+        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(base + (at ^ (c << 6))));
+        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(base + 8 * L::RB + (at ^ (c << 6) ^ 32)));
         out[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), b, out[c], 0, 0, 0);
       }
     }
   } else {
-    const int ln = lane & 31;
 #pragma unroll
     for (int r = 0; r < 16; r++)
 #pragma unroll
       for (int c = 0; c < L::NC; c++) {
-        const int col = c * 32 + ln;
-        out[c] = __builtin_amdgcn_mfma_f32_32x32x2f32((float)tile[L::off(acc_row(r, h), col >> 2) + (col & 3)], p[r], out[c], 0, 0, 0);
+        const int flip = ((8 * c) ^ ((r & 3) << 2) ^ (((r >> 2) & 1) << 1)) << 4;
+        const float v = *(const float*)((const char*)tile + (at ^ flip) + (tile_row + (r & 3) + 8 * (r >> 2)) * L::RB);
+        out[c] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[r], out[c], 0, 0, 0);
       }
   }
 }
@@ -140,25 +166,38 @@ __device__ inline void store_row(T* row, const f32x16* acc, int h, int dim, floa
     }
 }
 
-// R rows on their way from memory to an LDS tile through registers: thread -> (row, chunk), rows >= n and columns >= dim become zeros
-// (a row of another sequence may hold infinities or NaN: zero times those is NaN, so it must not reach a product even with probability zero)
-template <typename T, int DP, int R> struct Stage {
+// R rows of a tile, fetched straight into LDS (gemm_dma.h: 1 KiB a request, 64 lanes x 16 bytes in LDS order; the swizzle is applied to the
+// source address).  Rows that do not exist and columns behind the head dimension are requested out of range: the hardware writes zeros.  (A row
+// of another sequence may hold infinities or NaN, and zero times those is NaN: it must not reach a product even with probability zero.)
+// The lane's slot of a row is linear in the bits of the row's number, so request i differs from request 0 by an XOR and by whole rows, which go
+// into the instruction's scalar offset: one v_xad a request.
+template <typename T, int DP, int R> struct Fetch {
   using L = Tile<T, DP>;
-  static constexpr int NP = R * L::CPR / NT, RPP = NT / L::CPR;
-  Vec16<T> v[NP];
-  template <typename RowPtr>
-  __device__ inline void load(RowPtr rowptr, int r0, int n, int dim, int tid) {
-    const int chunk = tid % L::CPR, row = tid / L::CPR;
-#pragma unroll
-    for (int p = 0; p < NP; p++) {
-      const int r = r0 + row + p * RPP;
-      v[p] = (r < n && chunk * L::VEC < dim) ? ldg16(rowptr(r) + chunk * L::VEC) : zero16<T>();
-    }
+  static constexpr int NR = R * L::CPR / NT, RPR = 64 / L::CPR;      // requests of a wave, rows of a request
+  int wave, lrow;
+  int col;
+  unsigned rows, ldb;      // col: byte offset in the row (request 0), of the row, of a row step
+  __device__ inline void init(int wave_, int lane, long ld) {
+    wave = wave_;
+    lrow = wave * NR * RPR + lane / L::CPR;
+    ldb = (unsigned)(ld * (long)sizeof(T));
+    col = ((lane % L::CPR) ^ L::slot(lrow)) << 4;
+    rows = (unsigned)lrow * ldb;
   }
-  __device__ inline void store(T* tile, int tid) const {
-    const int chunk = tid % L::CPR, row = tid / L::CPR;
+  __device__ inline void get(T* tile, const T* base, int n, int dim) const {      // n: rows that exist
+    char* dst = (char*)tile + wave * NR * 1024;
+    int col = this->col;
+    opaque(col);
+    if (n >= R && dim == DP) {
 #pragma unroll
-    for (int p = 0; p < NP; p++) stg16(tile + L::off(row + p * RPP, chunk), v[p]);
+      for (int i = 0; i < NR; i++) dma_piece_at(base, dst + i * 1024, (unsigned)(col ^ (L::slot(i * RPR) << 4)) + rows, i * RPR * ldb);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NR; i++) {
+        const unsigned c = (unsigned)(col ^ (L::slot(i * RPR) << 4));
+        dma_piece_at(base, dst + i * 1024, (lrow + i * RPR < n && c < dim * sizeof(T)) ? c + rows + i * RPR * ldb : DMA_OOB, 0);
+      }
+    }
   }
 };
 
@@ -171,7 +210,7 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
   constexpr int KT = 32 * NB;
   __shared__ __attribute__((aligned(16))) T sK[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T sV[2][KT * DP];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, ln = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, ln = lane & 31;
   const int kh = blockIdx.x % a.kv_heads, ti = blockIdx.x / a.kv_heads;
   const int tile = a.tiles[2 * ti + 1];
   const Seq e = seq_of(a, a.tiles[2 * ti]);
@@ -183,8 +222,8 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
   const int lim = a.causal ? min(max(qi + 1 + off, 0), e.lk) : e.lk;      // the lane's row sees keys [0, lim)
   const auto limit = [&](int row) { return a.causal ? min(max(min(row, rows - 1) / a.group + 1 + off, 0), e.lk) : e.lk; };
   const int lim_lo = limit(r0), lim_hi = r0 < rows ? limit(r0 + 31) : 0;
-  const int kbeg = blockIdx.y * a.split_keys;
-  const int kend = min(limit(tile * BR + BR - 1), kbeg + a.split_keys);
+  const int kbeg = (int)min((long)blockIdx.y * a.split_keys, (long)0x7fffff00);
+  const int klast = limit(tile * BR + BR - 1), kend = blockIdx.y + 1 == gridDim.y ? klast : min(klast, kbeg + a.split_keys);
 
   Vec16<T> qf[L::NS];
   load_frag<T, DP>(qf, (const T*)a.Q + (long)(e.q0 + qi) * a.ldq + (long)(kh * a.group + rc % a.group) * a.hsq, h, dim, r < rows);
@@ -194,50 +233,55 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
 #pragma unroll
     for (int i = 0; i < 16; i++) o[c][i] = 0.f;
   float m = -INFINITY, mu = 0.f, l = 0.f;      // running maximum (log2 units), the same with 0 for -inf, the lane's share of the sum
-  const float c2 = a.scale * LOG2E;
+  // the maximum is taken over the unscaled products: a negative scale goes to the queries' signs.  (A scale of zero: all scores are 0, also those of
+  // infinite products, as 0 * q . k of finite numbers is)
+  const float c2 = fabsf(a.scale) * LOG2E;
+  if (a.scale < 0.f)
+#pragma unroll
+    for (int ks = 0; ks < L::NS; ks++)
+#pragma unroll
+      for (int j = 0; j < L::VEC; j++) qf[ks].v[j] = -qf[ks].v[j];
+  const int rows_at = L::rows_at(lane), cols_at = L::cols_at(lane);
   const T* kg = (const T*)a.K + (long)e.k0 * a.ldk + (long)kh * a.hsk;
   const T* vg = (const T*)a.V + (long)e.k0 * a.ldv + (long)kh * a.hsv;
-  const auto krow = [&](int key) { return kg + (long)key * a.ldk; };
-  const auto vrow = [&](int key) { return vg + (long)key * a.ldv; };
-  Stage<T, DP, KT> st_k, st_v;
+  Fetch<T, DP, KT> fk, fv;
+  fk.init(wave, lane, a.ldk);
+  fv.init(wave, lane, a.ldv);
   if (kbeg < kend) {
-    st_k.load(krow, kbeg, e.lk, dim, tid);
-    st_v.load(vrow, kbeg, e.lk, dim, tid);
-    st_k.store(sK[0], tid);
-    st_v.store(sV[0], tid);
+    fk.get(sK[0], kg + (long)kbeg * a.ldk, e.lk - kbeg, dim);
+    fv.get(sV[0], vg + (long)kbeg * a.ldv, e.lk - kbeg, dim);
   }
+  wait_vmcnt<0>();
   __syncthreads();
   int buf = 0;
   for (int kb = kbeg; kb < kend; kb += KT, buf ^= 1) {
     const bool more = kb + KT < kend;
-    if (more) {
-      st_k.load(krow, kb + KT, e.lk, dim, tid);
-      st_v.load(vrow, kb + KT, e.lk, dim, tid);
+    if (more) {      // (the barrier below: every wave is done with the other buffer)
+      fk.get(sK[buf ^ 1], kg + (long)(kb + KT) * a.ldk, e.lk - kb - KT, dim);
+      fv.get(sV[buf ^ 1], vg + (long)(kb + KT) * a.ldv, e.lk - kb - KT, dim);
     }
     if (kb < lim_hi) {      // (wave-uniform)
+      int at_r = rows_at + buf * KT * L::RB, at_c = cols_at + buf * KT * L::RB;
+      opaque(at_r);
+      opaque(at_c);
       f32x16 s[NB];
       float mt = -INFINITY;
 #pragma unroll
       for (int n = 0; n < NB; n++) {
 #pragma unroll
         for (int i = 0; i < 16; i++) s[n][i] = 0.f;
-        mma_rows<T, DP>(s[n], sK[buf] + n * 32 * DP, ln, h, qf);
+        mma_rows<T, DP>(s[n], sK[0], at_r, n * 32, qf);
       }
-      if (kb + KT <= lim_lo) {
+      if (kb + KT > lim_lo)
 #pragma unroll
         for (int n = 0; n < NB; n++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) { s[n][i] *= c2; mt = fmaxf(mt, s[n][i]); }
-      } else {
+          for (int i = 0; i < 16; i++) s[n][i] = kb + n * 32 + acc_row(i, h) < lim ? s[n][i] : -INFINITY;
 #pragma unroll
-        for (int n = 0; n < NB; n++)
+      for (int n = 0; n < NB; n++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            s[n][i] = kb + n * 32 + acc_row(i, h) < lim ? s[n][i] * c2 : -INFINITY;
-            mt = fmaxf(mt, s[n][i]);
-          }
-      }
-      mt = xor32_max(mt);
+        for (int i = 0; i < 16; i++) mt = fmaxf(mt, s[n][i]);
+      mt = xor32_max(mt) * c2;
       if (__any(mt > m + 8.f)) {
         // the accumulators follow the maximum only when it grew by more than 8 (log2 units): until then the probabilities are at most 2^8
         const float mn = fmaxf(m, mt);
@@ -253,27 +297,24 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
 #pragma unroll
       for (int n = 0; n < NB; n++) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) { s[n][i] = ex2(s[n][i] - mu); l += s[n][i]; }
-        mma_cols<T, DP>(o, sV[buf] + n * 32 * DP, s[n], lane);
+        for (int i = 0; i < 16; i++) { s[n][i] = ex2(s[n][i] * c2 - mu); l += s[n][i]; }
+        mma_cols<T, DP>(o, sV[0], at_c, n * 32, s[n]);
       }
     }
-    if (more) {
-      st_k.store(sK[buf ^ 1], tid);
-      st_v.store(sV[buf ^ 1], tid);
-    }
+    wait_vmcnt<0>();
     __syncthreads();
   }
   l = xor32_sum(l);
   if (r >= rows) return;
-  const long at = (long)kh * a.rows_q * a.group + (long)e.q0 * a.group + r;
+  const int hd = rc - qi * a.group;
   if (a.part_o) {
-    const long pr = (long)blockIdx.y * a.kv_heads * a.rows_q * a.group + at;
+    const long pr = ((long)blockIdx.y * a.kv_heads + kh) * a.rows_q * a.group + (long)e.q0 * a.group + r;
     store_row<float, DP>(a.part_o + pr * dim, o, h, dim, 1.f);
     if (h == 0) { a.part_ml[2 * pr] = m; a.part_ml[2 * pr + 1] = l; }
     return;
   }
-  store_row<T, DP>((T*)a.Out + (long)(e.q0 + qi) * a.ldo + (long)(kh * a.group + rc % a.group) * a.hso, o, h, dim, l == 0.f ? 0.f : 1.f / l);
-  if (h == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : m + __log2f(l);
+  store_row<T, DP>((T*)a.Out + (long)(e.q0 + qi) * a.ldo + (long)(kh * a.group + hd) * a.hso, o, h, dim, l == 0.f ? 0.f : 1.f / l);
+  if (h == 0 && a.lse) a.lse[(long)(kh * a.group + hd) * a.rows_q + e.q0 + qi] = l == 0.f ? -INFINITY : m + __log2f(l);
 }
 
 // the splits of a row meet: o = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.  One wave per row.
@@ -302,7 +343,7 @@ __global__ void __launch_bounds__(NT) packed_combine_kernel(const PackedArgs a, 
   T* op = (T*)a.Out + (rr / a.group) * a.ldo + (long)(kh * a.group + rr % a.group) * a.hso;
   if (lane < a.dim) op[lane] = Elem<T>::from_f(o0 * inv);
   if (lane + 64 < a.dim) op[lane + 64] = Elem<T>::from_f(o1 * inv);
-  if (lane == 0 && a.lse) a.lse[row] = l == 0.f ? -INFINITY : M + __log2f(l);
+  if (lane == 0 && a.lse) a.lse[(kh * a.group + rr % a.group) * a.rows_q + rr / a.group] = l == 0.f ? -INFINITY : M + __log2f(l);
 }
 
 // =====================================================================================================================
@@ -314,7 +355,7 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
   constexpr int KT = 32 * NB;
   __shared__ __attribute__((aligned(16))) T sK[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T sV[2][KT * DP];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, ln = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, ln = lane & 31;
   const int kh = blockIdx.x % a.kv_heads, ti = blockIdx.x / a.kv_heads;
   const int tile = a.tiles[2 * ti + 1];
   const Seq e = seq_of(a, a.tiles[2 * ti]);
@@ -328,7 +369,7 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
   const int lim_lo = limit(r0), lim_hi = r0 < rows ? limit(r0 + 31) : 0;
   const int kend = limit(tile * BR + BR - 1);
   const long row_g = e.q0 + qi, head = (long)kh * a.group + rc % a.group;
-  const long at = (long)kh * a.rows_q * a.group + (long)e.q0 * a.group + rc;
+  const long at = head * a.rows_q + row_g;
 
   Vec16<T> qf[L::NS], gf[L::NS];
   load_frag<T, DP>(qf, (const T*)a.Q + row_g * a.ldq + head * a.hsq, h, dim, r < rows);
@@ -351,6 +392,7 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
     if (h == 0 && r < rows) a.D[at] = Dr;
   }
   const float lse = a.lse[at], c2 = a.scale * LOG2E;
+  const int rows_at = L::rows_at(lane), cols_at = L::cols_at(lane);
   f32x16 dq[L::NC];
 #pragma unroll
   for (int c = 0; c < L::NC; c++)
@@ -358,101 +400,113 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
     for (int i = 0; i < 16; i++) dq[c][i] = 0.f;
   const T* kg = (const T*)a.K + (long)e.k0 * a.ldk + (long)kh * a.hsk;
   const T* vg = (const T*)a.V + (long)e.k0 * a.ldv + (long)kh * a.hsv;
-  const auto krow = [&](int key) { return kg + (long)key * a.ldk; };
-  const auto vrow = [&](int key) { return vg + (long)key * a.ldv; };
-  Stage<T, DP, KT> st_k, st_v;
+  Fetch<T, DP, KT> fk, fv;
+  fk.init(wave, lane, a.ldk);
+  fv.init(wave, lane, a.ldv);
   if (kend > 0) {
-    st_k.load(krow, 0, e.lk, dim, tid);
-    st_v.load(vrow, 0, e.lk, dim, tid);
-    st_k.store(sK[0], tid);
-    st_v.store(sV[0], tid);
+    fk.get(sK[0], kg, e.lk, dim);
+    fv.get(sV[0], vg, e.lk, dim);
   }
+  wait_vmcnt<0>();
   __syncthreads();
   int buf = 0;
   for (int kb = 0; kb < kend; kb += KT, buf ^= 1) {
     const bool more = kb + KT < kend;
-    if (more) {
-      st_k.load(krow, kb + KT, e.lk, dim, tid);
-      st_v.load(vrow, kb + KT, e.lk, dim, tid);
+    if (more) {      // (the barrier below: every wave is done with the other buffer)
+      fk.get(sK[buf ^ 1], kg + (long)(kb + KT) * a.ldk, e.lk - kb - KT, dim);
+      fv.get(sV[buf ^ 1], vg + (long)(kb + KT) * a.ldv, e.lk - kb - KT, dim);
     }
     if (kb < lim_hi) {
-      f32x16 s[NB], dp[NB];
-#pragma unroll
-      for (int n = 0; n < NB; n++) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[n][i] = dp[n][i] = 0.f;
-        mma_rows<T, DP>(s[n], sK[buf] + n * 32 * DP, ln, h, qf);
-        mma_rows<T, DP>(dp[n], sV[buf] + n * 32 * DP, ln, h, gf);
-      }
+      int at_r = rows_at + buf * KT * L::RB, at_c = cols_at + buf * KT * L::RB;
+      opaque(at_r);
+      opaque(at_c);
       const bool whole = kb + KT <= lim_lo;
+      const auto probs = [&](int n, f32x16& s, f32x16& dp) {      // P and dP of 32 keys
 #pragma unroll
-      for (int n = 0; n < NB; n++)
+        for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
+        mma_rows<T, DP>(s, sK[0], at_r, n * 32, qf);
+        mma_rows<T, DP>(dp, sV[0], at_r, n * 32, gf);
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          // (the exponential of a selected argument, so that the compiler makes no branch per score)
-          const float x = s[n][i] * c2 - lse;
-          s[n][i] = ex2((whole | (kb + n * 32 + acc_row(i, h) < lim)) ? x : -INFINITY);
-        }
+        for (int i = 0; i < 16; i++) s[i] = s[i] * c2 - lse;
+        if (!whole)
+#pragma unroll
+          for (int i = 0; i < 16; i++) s[i] = kb + n * 32 + acc_row(i, h) < lim ? s[i] : -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = ex2(s[i]);
+      };
+      f32x16 s, dp;
       if (one_tile) {
+        for (int n = 0; n < NB; n++) {
+          probs(n, s, dp);
 #pragma unroll
-        for (int n = 0; n < NB; n++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) Dr += s[n][i] * dp[n][i];
+          for (int i = 0; i < 16; i++) Dr += s[i] * dp[i];
+        }
         Dr = xor32_sum(Dr);
       }
 #pragma unroll
       for (int n = 0; n < NB; n++) {
+        probs(n, s, dp);
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[n][i] = s[n][i] * (dp[n][i] - Dr) * a.scale;
-        mma_cols<T, DP>(dq, sK[buf] + n * 32 * DP, s[n], lane);
+        for (int i = 0; i < 16; i++) s[i] = s[i] * (dp[i] - Dr);      // (the scale follows at the end)
+        mma_cols<T, DP>(dq, sK[0], at_c, n * 32, s);
       }
     }
-    if (more) {
-      st_k.store(sK[buf ^ 1], tid);
-      st_v.store(sV[buf ^ 1], tid);
-    }
+    wait_vmcnt<0>();
     __syncthreads();
   }
   if (r >= rows) return;
   if (one_tile && h == 0) a.D[at] = Dr;
-  store_row<T, DP>((T*)a.dQ + row_g * a.lddq + head * a.hsdq, dq, h, dim, 1.f);
+  store_row<T, DP>((T*)a.dQ + row_g * a.lddq + head * a.hsdq, dq, h, dim, a.scale);
 }
 
 // =====================================================================================================================
-// backward 2: dK, dV.  grid (kv_heads * key tiles); a block owns 128 keys, 32 a wave; the group's query rows stream through LDS.
+// backward 2: dK, dV.  grid (kv_heads * key tiles, row parts); a block owns 64 keys, the group's query rows stream through LDS 64 at a time: the
+// waves are 2 groups of 32 keys x 2 halves of the rows, the halves meet in LDS at the end.  (128 keys a block, 32 rows at a time reads LDS as
+// much for each product, but a 5000-row sequence of four heads was one chain of 625 steps in 568 blocks.)
+// A key tile with more than `piece` rows is cut into parts, a block each, whose float sums meet in packed_parts_kernel in order.
 // =====================================================================================================================
+struct Parts { int begin, end, n, first, per; };
+// The rows of a key tile, head by head: `per` steps of 64 queries from the first query that sees its first key, for each head of the group.
+// Steps [begin, end) of part y, and the number of parts.
+__device__ inline Parts parts_of(const PackedArgs& a, const Seq& e, int tile, int y) {
+  Parts p;
+  p.first = a.causal ? min(max(tile * BK - (e.lk - e.lq), 0), e.lq) : 0;
+  p.per = (e.lq - p.first + 63) / 64;
+  const int steps = p.per * a.group;
+  p.n = min(max((steps + a.piece - 1) / a.piece, 1), a.parts);
+  p.begin = (int)min((long)y * a.piece, (long)steps);
+  p.end = y == p.n - 1 ? steps : min(p.begin + a.piece, steps);
+  return p;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_kernel(const PackedArgs a) {
   using L = Tile<T, DP>;
-  constexpr int RT = 32;
+  constexpr int RT = 64;
   __shared__ __attribute__((aligned(16))) T sQ[2][RT * DP];
   __shared__ __attribute__((aligned(16))) T sG[2][RT * DP];
-  __shared__ __attribute__((aligned(16))) float sL[2][RT];
-  __shared__ __attribute__((aligned(16))) float sD[2][RT];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, ln = lane & 31;
+  __shared__ __attribute__((aligned(16))) float sS[2][2][RT];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, ln = lane & 31;
   const int kh = blockIdx.x % a.kv_heads, ti = blockIdx.x / a.kv_heads;
   const int tile = a.tiles[2 * ti + 1];
   const Seq e = seq_of(a, a.tiles[2 * ti]);
-  const int rows = e.lq * a.group, dim = a.dim;
-  const int k0 = tile * BR + wave * 32, key = k0 + ln, kc = min(key, e.lk - 1);
-  if (tile < 0 || tile * BR >= e.lk) return;
+  const int dim = a.dim;
+  const int kw = wave & 1, rw = wave >> 1;
+  const int k0 = tile * BK + kw * 32, key = k0 + ln, kc = min(key, e.lk - 1);
+  if (tile < 0 || tile * BK >= e.lk) return;
+  const Parts part = parts_of(a, e, tile, blockIdx.y);
+  if ((int)blockIdx.y >= part.n) return;      // (uniform)
   const int off = e.lk - e.lq;
-  // rows >= first(key) see the key: query >= key - off, row = query * group
-  const auto first = [&](int k) { return a.causal ? max(k - off, 0) * a.group : 0; };
-  const int rmin = first(key), rbeg = first(tile * BR) / RT * RT;
-  const int wbeg = first(k0), wall = first(k0 + 31);      // the wave's first row at all, its first row that sees all its keys
-  const T* qg = (const T*)a.Q + (long)e.q0 * a.ldq + (long)kh * a.group * a.hsq;
-  const T* gg = (const T*)a.dO + (long)e.q0 * a.lddo + (long)kh * a.group * a.hsdo;
-  const auto qrow = [&](int r) { const int q = r / a.group; return qg + (long)q * a.ldq + (long)(r - q * a.group) * a.hsq; };
-  const auto grow = [&](int r) { const int q = r / a.group; return gg + (long)q * a.lddo + (long)(r - q * a.group) * a.hsdo; };
-  const float* lg = a.lse + (long)kh * a.rows_q * a.group + (long)e.q0 * a.group;
-  const float* dg = a.D + (long)kh * a.rows_q * a.group + (long)e.q0 * a.group;
+  const int qmin = a.causal ? key - off : 0;      // the lane's key is seen by queries >= qmin
+  const int wbeg = a.causal ? k0 - off : 0, wall = a.causal ? k0 + 31 - off : 0;      // the wave's first query at all, its first that sees all its keys
+  const long hd0 = (long)kh * a.group;
   // rows that do not exist, and rows without a key, take no probability: 2^(s - inf) = 0
-  const auto stat = [&](int r) {
-    if (tid < RT) { const float v = r + tid < rows ? lg[r + tid] : INFINITY; return v == -INFINITY ? INFINITY : v; }
-    return (tid < 2 * RT && r + tid - RT < rows) ? dg[r + tid - RT] : 0.f;
+  const auto stat = [&](int hd, int q) {      // wave 0: lse, wave 1: D
+    float v = wave == 0 ? INFINITY : 0.f;
+    if (wave < 2 && q + lane < e.lq) v = ((wave == 0 ? a.lse : a.D) + (hd0 + hd) * a.rows_q + e.q0 + q)[lane];
+    return v == -INFINITY ? INFINITY : v;
   };
-  const auto stat_put = [&](int b, float v) { if (tid < RT) sL[b][tid] = v; else if (tid < 2 * RT) sD[b][tid - RT] = v; };
+  const auto stat_put = [&](int b, float v) { if (wave < 2) sS[b][wave][lane] = v; };
 
   Vec16<T> kf[L::NS], vf[L::NS];
   load_frag<T, DP>(kf, (const T*)a.K + (long)(e.k0 + kc) * a.ldk + (long)kh * a.hsk, h, dim, key < e.lk);
@@ -463,60 +517,121 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_ke
 #pragma unroll
     for (int i = 0; i < 16; i++) dk[c][i] = dv[c][i] = 0.f;
   const float c2 = a.scale * LOG2E;
-  Stage<T, DP, RT> st_q, st_g;
+  Fetch<T, DP, RT> fq, fg;
+  fq.init(wave, lane, a.ldq);
+  fg.init(wave, lane, a.lddo);
+  const auto fetch = [&](int b, int hd, int q) {
+    fq.get(sQ[b], (const T*)a.Q + (long)(e.q0 + q) * a.ldq + (hd0 + hd) * a.hsq, e.lq - q, dim);
+    fg.get(sG[b], (const T*)a.dO + (long)(e.q0 + q) * a.lddo + (hd0 + hd) * a.hsdo, e.lq - q, dim);
+  };
+  const int rows_at = L::rows_at(lane) + rw * 32 * L::RB, cols_at = L::cols_at(lane) + rw * 32 * L::RB;
   float rs = 0.f;
-  if (rbeg < rows) {
-    st_q.load(qrow, rbeg, rows, dim, tid);
-    st_g.load(grow, rbeg, rows, dim, tid);
-    st_q.store(sQ[0], tid);
-    st_g.store(sG[0], tid);
-    stat_put(0, stat(rbeg));
+  int hd = part.begin / max(part.per, 1), q = part.first + (part.begin - hd * part.per) * RT;
+  if (part.begin < part.end) {
+    fetch(0, hd, q);
+    stat_put(0, stat(hd, q));
   }
+  wait_vmcnt<0>();
   __syncthreads();
   int buf = 0;
-  for (int rb = rbeg; rb < rows; rb += RT, buf ^= 1) {
-    const bool more = rb + RT < rows;
+  for (int st = part.begin; st < part.end; st++, buf ^= 1) {
+    const bool more = st + 1 < part.end;
+    const int q_now = q;
+    q += RT;
+    if (q >= e.lq) { q = part.first; hd++; }
     if (more) {
-      st_q.load(qrow, rb + RT, rows, dim, tid);
-      st_g.load(grow, rb + RT, rows, dim, tid);
-      rs = stat(rb + RT);
+      rs = stat(hd, q);
+      fetch(buf ^ 1, hd, q);
     }
-    if (k0 < e.lk && rb + RT > wbeg) {
+    const int r0 = q_now + rw * 32;
+    if (k0 < e.lk && r0 + 32 > wbeg && r0 < e.lq) {
+      int at_r = rows_at + buf * RT * L::RB, at_c = cols_at + buf * RT * L::RB;
+      opaque(at_r);
+      opaque(at_c);
       f32x16 s, dp;
 #pragma unroll
       for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
-      mma_rows<T, DP>(s, sQ[buf], ln, h, kf);
-      mma_rows<T, DP>(dp, sG[buf], ln, h, vf);
-      float lr[16], dr[16];
+      mma_rows<T, DP>(s, sQ[0], at_r, 0, kf);
+      mma_rows<T, DP>(dp, sG[0], at_r, 0, vf);
+      if (r0 < wall)
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = r0 + acc_row(i, h) >= qmin ? s[i] * c2 : -INFINITY;
+      else
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] *= c2;
 #pragma unroll
       for (int g = 0; g < 4; g++) {
-        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&sL[buf][8 * g + 4 * h]), d4 = *reinterpret_cast<const f32x4*>(&sD[buf][8 * g + 4 * h]);
+        const int at = rw * 32 + 8 * g + 4 * h;
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&sS[buf][0][at]), d4 = *reinterpret_cast<const f32x4*>(&sS[buf][1][at]);
 #pragma unroll
-        for (int j = 0; j < 4; j++) { lr[4 * g + j] = l4[j]; dr[4 * g + j] = d4[j]; }
+        for (int j = 0; j < 4; j++) {
+          const int i = 4 * g + j;
+          s[i] = ex2(s[i] - l4[j]);
+          dp[i] = s[i] * (dp[i] - d4[j]);      // (the scale follows at the end)
+        }
       }
-      const bool whole = rb >= wall;
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const float x = s[i] * c2 - lr[i];
-        s[i] = ex2((whole | (rb + acc_row(i, h) >= rmin)) ? x : -INFINITY);
-        dp[i] = s[i] * (dp[i] - dr[i]) * a.scale;
-      }
-      mma_cols<T, DP>(dv, sG[buf], s, lane);
-      mma_cols<T, DP>(dk, sQ[buf], dp, lane);
+      mma_cols<T, DP>(dv, sG[0], at_c, 0, s);
+      mma_cols<T, DP>(dk, sQ[0], at_c, 0, dp);
     }
-    if (more) {
-      st_q.store(sQ[buf ^ 1], tid);
-      st_g.store(sG[buf ^ 1], tid);
-      stat_put(buf ^ 1, rs);
-    }
+    if (more) stat_put(buf ^ 1, rs);
+    wait_vmcnt<0>();
     __syncthreads();
   }
-  if (key >= e.lk) return;
-  store_row<T, DP>((T*)a.dK + (long)(e.k0 + key) * a.lddk + (long)kh * a.hsdk, dk, h, dim, 1.f);
+  // the second half of the rows joins the first: 16 * NC floats of a lane through LDS, dK and then dV
+  float* meet = reinterpret_cast<float*>(sQ) + kw * 16 * L::NC * 64;      // (2 x 16 NC x 64 floats: sQ holds as many bytes)
+  static_assert(sizeof(T) * 2 * RT * DP >= 2 * 16 * L::NC * 64 * 4, "room for the halves");
+#pragma unroll
+  for (int m = 0; m < 2; m++) {
+    f32x16* acc = m == 0 ? dk : dv;
+    if (rw == 1)
+#pragma unroll
+      for (int c = 0; c < L::NC; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) meet[(c * 16 + i) * 64 + lane] = acc[c][i];
+    __syncthreads();
+    if (rw == 0)
+#pragma unroll
+      for (int c = 0; c < L::NC; c++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) acc[c][i] += meet[(c * 16 + i) * 64 + lane];
+    __syncthreads();
+  }
+  if (rw == 1 || key >= e.lk) return;
+  if (part.n > 1) {
+    float* p = a.part_o + (((long)blockIdx.y * a.kv_heads + kh) * a.rows_k + e.k0 + key) * 2 * dim;
+    store_row<float, DP>(p, dk, h, dim, a.scale);
+    store_row<float, DP>(p + dim, dv, h, dim, 1.f);
+    return;
+  }
+  store_row<T, DP>((T*)a.dK + (long)(e.k0 + key) * a.lddk + (long)kh * a.hsdk, dk, h, dim, a.scale);
   store_row<T, DP>((T*)a.dV + (long)(e.k0 + key) * a.lddv + (long)kh * a.hsdv, dv, h, dim, 1.f);
 }
 
+// dK, dV of the key tiles in several parts, summed in order.  Same grid as above without the parts.
+template <typename T>
+__global__ void __launch_bounds__(NT) packed_parts_kernel(const PackedArgs a) {
+  const int kh = blockIdx.x % a.kv_heads, ti = blockIdx.x / a.kv_heads;
+  const int tile = a.tiles[2 * ti + 1];
+  const Seq e = seq_of(a, a.tiles[2 * ti]);
+  if (tile < 0 || tile * BK >= e.lk) return;
+  const int n = parts_of(a, e, tile, 0).n;
+  if (n == 1) return;
+  const int keys = min(BK, e.lk - tile * BK), per = 2 * a.dim / 4;
+  for (int i = threadIdx.x; i < keys * per; i += NT) {
+    const int k = i / per, c = (i - k * per) * 4;
+    const long key = e.k0 + tile * BK + k;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int y = 0; y < n; y++) v += *reinterpret_cast<const f32x4*>(a.part_o + (((long)y * a.kv_heads + kh) * a.rows_k + key) * 2 * a.dim + c);
+    T* p = c < a.dim ? (T*)a.dK + key * a.lddk + (long)kh * a.hsdk + c : (T*)a.dV + key * a.lddv + (long)kh * a.hsdv + c - a.dim;
+#pragma unroll
+    for (int j = 0; j < 4; j++) p[j] = Elem<T>::from_f(v[j]);
+  }
+}
+
 bool rows16(const void* p, int64_t ld, int64_t hs, int vec) { return ((uintptr_t)p % 16) == 0 && ld % vec == 0 && hs % vec == 0; }
+
+// the rows of one tile lie within 2^31 bytes (32-bit offsets of the LDS requests)
+bool near(int64_t ld, int dtype) { return ld >= 0 && ld * 64 * (dtype == CROG_BF16 ? 2 : 4) < 0x7fff0000; }
 
 int check_common(const char* what, int dtype, int seqs, int rows_q, int rows_k, int kv_heads, int group, int head_dim, int n_tiles, const int* cu_q,
                  const int* cu_k, const int* tiles) {
@@ -539,6 +654,7 @@ extern "C" int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64
   const int vec = dtype == CROG_BF16 ? 8 : 4;
   CROG_CHECK_ARG(rows16(Q, ldq, hsq, vec) && rows16(K, ldk, hsk, vec) && rows16(V, ldv, hsv, vec) && rows16(O, ldo, hso, vec) && Q && K && V && O,
                  "packed_attn_fwd: heads of Q / K / V / O must start at 16-byte boundaries");
+  CROG_CHECK_ARG(near(ldk, dtype) && near(ldv, dtype), "packed_attn_fwd: 64 key rows must lie within 2 GiB");
   CROG_CHECK_ARG(splits >= 1 && splits <= 65535 && (splits == 1 || (partial && split_keys > 0 && split_keys % 64 == 0)),
                  "packed_attn_fwd: %d splits need a workspace and a multiple of 64 keys each (got %d)", splits, split_keys);
   if (n_tiles == 0) return CROG_OK;
@@ -573,13 +689,17 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
                                     const float* lse, float* D, void* dQ, int64_t lddq, int64_t hsdq, void* dK, int64_t lddk, int64_t hsdk, void* dV,
                                     int64_t lddv, int64_t hsdv, const int* cu_q, const int* cu_k, const int* row_tiles, int n_row_tiles,
                                     const int* key_tiles, int n_key_tiles, int seqs, int rows_q, int rows_k, int kv_heads, int group, int head_dim,
-                                    float scale, int causal, crog_stream_t stream) {
+                                    float scale, int causal, int parts, int part_steps, float* partial, crog_stream_t stream) {
   if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_row_tiles, cu_q, cu_k, row_tiles)) return rc;
   if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_key_tiles, cu_q, cu_k, key_tiles)) return rc;
   const int vec = dtype == CROG_BF16 ? 8 : 4;
   CROG_CHECK_ARG(rows16(Q, ldq, hsq, vec) && rows16(K, ldk, hsk, vec) && rows16(V, ldv, hsv, vec) && rows16(O, ldo, hso, vec) && rows16(dO, lddo, hsdo, vec) &&
                  rows16(dQ, lddq, hsdq, vec) && rows16(dK, lddk, hsdk, vec) && rows16(dV, lddv, hsdv, vec) && Q && K && V && O && dO && lse && D && dQ && dK && dV,
                  "packed_attn_bwd: heads of Q / K / V / O / dO and the gradients must start at 16-byte boundaries");
+  CROG_CHECK_ARG(parts >= 1 && parts <= 65535 && (parts == 1 || (part_steps > 0 && partial)),
+                 "packed_attn_bwd: %d parts need a workspace and a number of steps each (got %d)", parts, part_steps);
+  CROG_CHECK_ARG(near(ldk, dtype) && near(ldv, dtype) && near(ldq, dtype) && near(lddo, dtype),
+                 "packed_attn_bwd: 64 rows must lie within 2 GiB");
   PackedArgs a{};
   a.Q = Q; a.K = K; a.V = V; a.O = O; a.dO = dO; a.lse = const_cast<float*>(lse); a.D = D; a.dQ = dQ; a.dK = dK; a.dV = dV;
   a.ldq = ldq; a.hsq = hsq; a.ldk = ldk; a.hsk = hsk; a.ldv = ldv; a.hsv = hsv; a.ldo = ldo; a.hso = hso; a.lddo = lddo; a.hsdo = hsdo;
@@ -601,7 +721,10 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
   }
   if (n_key_tiles > 0) {
     a.tiles = key_tiles;
-    const unsigned n = (unsigned)(n_key_tiles * kv_heads);
+    a.parts = parts;
+    a.piece = parts > 1 ? part_steps : 0x7fffff00;
+    a.part_o = partial;
+    const dim3 n((unsigned)(n_key_tiles * kv_heads), parts);
     if (dtype == CROG_BF16) {
       if (head_dim <= 64) packed_bwd_dkdv_kernel<bf16, 64><<<n, NT, 0, s>>>(a);
       else packed_bwd_dkdv_kernel<bf16, 128><<<n, NT, 0, s>>>(a);
@@ -610,6 +733,11 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
       else packed_bwd_dkdv_kernel<float, 128><<<n, NT, 0, s>>>(a);
     }
     CROG_LAUNCH_CHECK();
+    if (parts > 1) {
+      if (dtype == CROG_BF16) packed_parts_kernel<bf16><<<n.x, NT, 0, s>>>(a);
+      else packed_parts_kernel<float><<<n.x, NT, 0, s>>>(a);
+      CROG_LAUNCH_CHECK();
+    }
   }
   return CROG_OK;
 }

@@ -760,8 +760,10 @@ def same_device(*ts):
 
 def heads16(t: torch.Tensor) -> torch.Tensor:
     """`t` [rows, heads, dim] if every head starts on a 16-byte boundary and its columns are adjacent, else a contiguous copy."""
+    s0, s1, s2 = t.stride()
     vec = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % vec == 0 and t.stride(1) % vec == 0 and t.data_ptr() % 16 == 0:
+    # (a tile of 64 rows is addressed with 32-bit offsets: rows or heads further apart than that are copied too)
+    if s2 == 1 and s0 % vec == 0 and s1 % vec == 0 and t.data_ptr() % 16 == 0 and s0 < 1 << 22 and s1 * t.shape[1] < 1 << 27:
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -780,12 +782,14 @@ def packed_attn_fwd(q, k, v, o, lse, rows, scale):
 
 def packed_attn_bwd(q, k, v, o, do, lse, D, dq, dk, dv, rows, scale):
     kv, dim = k.shape[1], k.shape[2]
+    parts, piece = rows.parts(kv)
+    ws = torch.empty(parts * kv * rows.rows_k * 2 * dim, device=q.device, dtype=torch.float32) if parts > 1 else None
     check(lib().crog_packed_attn_bwd(dcode(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                                      v.stride(1), o.data_ptr(), o.stride(0), o.stride(1), do.data_ptr(), do.stride(0), do.stride(1), ptr(lse), ptr(D),
                                      dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1), dv.data_ptr(), dv.stride(0),
                                      dv.stride(1), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr, rows.n_row_tiles, rows.key_tiles_ptr,
-                                     rows.n_key_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, stream()),
-          "packed_attn_bwd")
+                                     rows.n_key_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, parts, piece, ptr(ws),
+                                     stream()), "packed_attn_bwd")
 
 
 def rotary(q, k, q_out, k_out, positions, axes, inverse=False):

@@ -12,11 +12,13 @@ from typing import Optional, Sequence
 import numpy as np
 import torch
 
-TILE = 128      # rows (query rows x heads of a group) or keys of a block of csrc/packed_attn.hip
+TILE = 128      # rows (query rows x heads of a group) of a forward / dQ block of csrc/packed_attn.hip
+KEY_TILE = 64   # keys of a dK / dV block
 # Key splits of the forward pass: with fewer blocks than this, a long key axis is cut into pieces so that every CU has work (256 CUs, two blocks
 # each); a piece is at least SPLIT_MIN keys.
 FILL_BLOCKS = 512
 SPLIT_MIN = 256
+STEP, PART_MIN = 64, 16      # queries of a dK / dV step; steps of a part at least
 
 
 def _lengths(name: str, lengths: Sequence[int]) -> np.ndarray:
@@ -32,13 +34,15 @@ def _lengths(name: str, lengths: Sequence[int]) -> np.ndarray:
     return np.asarray(out, dtype=np.int64)
 
 
-def _tiles(rows: np.ndarray, cost) -> np.ndarray:
-    """[(sequence, tile)] of all 128-row tiles, the costliest first (a late long one would leave the device waiting for a single block)."""
-    n = (rows + TILE - 1) // TILE
+def _tiles(rows: np.ndarray, size: int, cost):
+    """[(sequence, tile)] of all tiles of `size` rows, the costliest first (a late long one would leave the device waiting for a single block),
+    and their costs."""
+    n = (rows + size - 1) // size
     seq = np.repeat(np.arange(len(rows)), n)
     tile = np.arange(len(seq)) - np.repeat(np.cumsum(n) - n, n)
-    order = np.argsort(-cost(seq, tile), kind="stable")
-    return np.stack([seq[order], tile[order]], 1)
+    c = cost(seq, tile)
+    order = np.argsort(-c, kind="stable")
+    return np.stack([seq[order], tile[order]], 1), c[order]
 
 
 class PackedRows:
@@ -69,10 +73,12 @@ class PackedRows:
             last = np.minimum(t * TILE + TILE - 1, lq[s] * g - 1) // g
             return np.clip(last + 1 + lk[s] - lq[s], 0, lk[s]) if c else lk[s]
 
-        def key_cost(s, t):      # rows that see the tile's first key
-            return (lq[s] - np.clip(t * TILE - (lk[s] - lq[s]), 0, lq[s])) * g if c else lq[s] * g
+        def key_cost(s, t):      # steps of the tile: 64 queries of one head each, from the first that sees its first key
+            first = np.clip(t * KEY_TILE - (lk[s] - lq[s]), 0, lq[s]) if c else 0
+            return (lq[s] - first + STEP - 1) // STEP * g
 
-        rt, kt = _tiles(lq * g, row_cost), _tiles(lk, key_cost)
+        (rt, _), (kt, kc) = _tiles(lq * g, TILE, row_cost), _tiles(lk, KEY_TILE, key_cost)
+        self.key_work, self.key_most = int(kc.sum()), int(kc.max()) if len(kc) else 0
         self.n_row_tiles, self.n_key_tiles = len(rt), len(kt)
         zero = np.zeros(1, dtype=np.int64)
         parts = [np.concatenate([zero, np.cumsum(lq)]), np.concatenate([zero, np.cumsum(lk)]), rt.reshape(-1), kt.reshape(-1)]
@@ -95,6 +101,15 @@ class PackedRows:
         piece = -(-self.max_k // n)
         piece = -(-piece // 64) * 64
         return -(-self.max_k // piece), piece
+
+
+    def parts(self, kv_heads: int):
+        """(parts, steps of a part) of the dK / dV pass: a block walks over every query that sees its keys - 16384 queries of 8 heads are 2048
+        steps -, so a tile's steps are cut where one chain would be longer than the device's share of all of them."""
+        piece = max(PART_MIN, -(-self.key_work * kv_heads // FILL_BLOCKS))
+        if self.key_most <= piece:
+            return 1, 0
+        return -(-self.key_most // piece), piece
 
 
 class RotaryAxes:

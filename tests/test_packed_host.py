@@ -5,7 +5,7 @@ import torch
 
 from crog_amd import _lib
 from crog_amd import functional as Fn
-from crog_amd.packed import SPLIT_MIN, TILE, PackedRows, RotaryAxes
+from crog_amd.packed import KEY_TILE, SPLIT_MIN, TILE, PackedRows, RotaryAxes
 
 
 def tables(p):
@@ -24,7 +24,7 @@ def test_plan_covers_every_row_and_key_once(causal, group):
     assert cu_q.tolist() == [0] + np.cumsum(lq).tolist() and cu_k.tolist() == [0] + np.cumsum(lk).tolist()
     assert (p.rows_q, p.rows_k, p.max_k) == (sum(lq), sum(lk), 4000)
     want_r = {(s, t) for s, n in enumerate(lq) for t in range(-(-n * group // TILE))}
-    want_k = {(s, t) for s, n in enumerate(lk) for t in range(-(-n // TILE))}
+    want_k = {(s, t) for s, n in enumerate(lk) for t in range(-(-n // KEY_TILE))}
     assert len(rt) == len(want_r) and {tuple(r) for r in rt.tolist()} == want_r
     assert len(kt) == len(want_k) and {tuple(r) for r in kt.tolist()} == want_k
     # the costliest block first: the keys a row tile sees do not grow along the list
@@ -47,6 +47,20 @@ def test_splits_cover_the_keys(seqs, keys, kv):
         assert seqs * kv >= 512 or keys <= SPLIT_MIN
     else:
         assert piece % 64 == 0 and n * piece >= keys > (n - 1) * piece and piece >= SPLIT_MIN // 2
+
+
+@pytest.mark.parametrize("lq,lk,group,kv,causal", [([5000, 300], None, 4, 4, True), ([4096], None, 8, 1, True), ([16384], [20], 1, 8, False), ([20] * 32, None, 1, 8, True),
+                                                   ([3000], [100], 2, 1, True)])
+def test_parts_cover_the_rows(lq, lk, group, kv, causal):
+    p = PackedRows(lq, lk, group=group, causal=causal, device="cpu")
+    n, piece = p.parts(kv)
+    # the steps of a sequence's first key, seen by all its queries but those that see nothing
+    most = max(-(-(q - max(0, q - k) * causal) // 64) * group for q, k in zip(lq, lk or lq))
+    assert p.key_most == most
+    if n == 1:
+        assert most <= max(16, -(-p.key_work * kv // 512))
+    else:
+        assert piece >= 16 and n * piece >= most > (n - 1) * piece
 
 
 @pytest.mark.parametrize("make,error", [
@@ -144,8 +158,8 @@ def test_c_entries_refuse_before_any_launch():
     for kw in bad:
         assert fwd(**kw) == -1, kw
         assert b"packed_attn_fwd" in lib.crog_last_error()
-    args = [1] + [p, 64, 64] * 5 + [p, p] + [p, 64, 64] * 3 + [p, p, p, 1, p, 1, 1, 8, 8, 1, 1, 64, 1.0, 0, None]
-    for at, v in ((0, 2), (1, None), (13, p + 8), (16, None), (17, None), (20, 4), (27, None), (38, 60)):
+    args = [1] + [p, 64, 64] * 5 + [p, p] + [p, 64, 64] * 3 + [p, p, p, 1, p, 1, 1, 8, 8, 1, 1, 64, 1.0, 0, 1, 0, None, None]
+    for at, v in ((0, 2), (1, None), (13, p + 8), (16, None), (17, None), (20, 4), (27, None), (38, 60), (41, 2), (41, 0), (2, 1 << 40), (5, 1 << 30)):
         assert lib.crog_packed_attn_bwd(*args[:at], v, *args[at + 1:]) == -1, at
     r = [1, p, 64, 64, p, 64, 64, p, 64, 64, p, 64, 64, p, 1, 4, p, p, 8, 1, 1, 64, 32, 1, 0, 0, None]
     for at, v in ((0, 2), (1, None), (13, None), (14, 0), (15, 2), (16, None), (18, -1), (22, 33), (22, 0), (23, 0)):
