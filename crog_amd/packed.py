@@ -13,12 +13,12 @@ import numpy as np
 import torch
 
 TILE = 128      # rows (query rows x heads of a group) of a forward / dQ block of csrc/packed_attn.hip
-KEY_TILE = 64   # keys of a dK / dV block
+KEY_TILE = 128  # keys of a dK / dV block
 # Key splits of the forward pass: with fewer blocks than this, a long key axis is cut into pieces so that every CU has work (256 CUs, two blocks
 # each); a piece is at least SPLIT_MIN keys.
 FILL_BLOCKS = 512
 SPLIT_MIN = 256
-STEP, PART_MIN = 64, 16      # queries of a dK / dV step; steps of a part at least
+STEP, PART_MIN = 32, 32      # queries of a dK / dV step; steps of a part at least
 
 
 def _lengths(name: str, lengths: Sequence[int]) -> np.ndarray:
@@ -73,9 +73,9 @@ class PackedRows:
             last = np.minimum(t * TILE + TILE - 1, lq[s] * g - 1) // g
             return np.clip(last + 1 + lk[s] - lq[s], 0, lk[s]) if c else lk[s]
 
-        def key_cost(s, t):      # steps of the tile: 64 queries of one head each, from the first that sees its first key
+        def key_cost(s, t):      # steps of the tile: 32 queries of one head each, from the block that first sees its first key to the last
             first = np.clip(t * KEY_TILE - (lk[s] - lq[s]), 0, lq[s]) if c else 0
-            return (lq[s] - first + STEP - 1) // STEP * g
+            return ((lq[s] + STEP - 1) // STEP - first // STEP) * g
 
         (rt, _), (kt, kc) = _tiles(lq * g, TILE, row_cost), _tiles(lk, KEY_TILE, key_cost)
         self.key_work, self.key_most = int(kc.sum()), int(kc.max()) if len(kc) else 0
@@ -104,7 +104,7 @@ class PackedRows:
 
 
     def parts(self, kv_heads: int):
-        """(parts, steps of a part) of the dK / dV pass: a block walks over every query that sees its keys - 16384 queries of 8 heads are 2048
+        """(parts, steps of a part) of the dK / dV pass: a block walks over every query that sees its keys - 16384 queries of 8 heads are 4096
         steps -, so a tile's steps are cut where one chain would be longer than the device's share of all of them."""
         piece = max(PART_MIN, -(-self.key_work * kv_heads // FILL_BLOCKS))
         if self.key_most <= piece:

@@ -614,11 +614,12 @@ int crog_preprocess_u8(const uint8_t* img, const uint8_t* masks, int B, int H, i
  * (bf16) or 4 (fp32) up to 128; head kv * group + g of Q reads head kv of K / V.  Sequence s owns query rows cu_q[s] .. cu_q[s + 1] - 1 and key
  * rows cu_k[s] .. (device int32 tables of seqs + 1 entries, not decreasing, at most rows_q / rows_k).  causal: query i of Lq sees keys
  * j <= i + Lk - Lq (the ends aligned; a query that sees none gives zeros).  tiles: device int32 pairs (sequence, tile): blocks of 128 of the
- * sequence's Lq * group rows (forward, dQ: row_tiles) or of 64 keys (key_tiles), each exactly once, in the order in which they should start.
- * lse (may be NULL in the forward) and D: [kv_heads * group][rows_q] floats, base-2 logarithms, the forward's for the backward.
+ * sequence's Lq * group rows (forward, dQ: row_tiles) or of 128 keys (key_tiles), each exactly once, in the order in which they should start.
+ * lse (may be NULL in the forward) and D: [kv_heads * group][rows_q] floats: the forward's base-2 log-sum-exp (+inf for a row without a key) for
+ * the backward, and scratch of the backward (rowsum(dO * O)).
  * splits > 1: the keys of a row are walked in `splits` pieces of split_keys (a multiple of 64; splits * split_keys >= the longest key
  * sequence) that meet in a second launch; partial: splits * kv_heads * rows_q * group * (head_dim + 2) floats.
- * parts > 1: a key tile's steps - 64 queries of one head each, from the first that sees it - are walked in up to `parts` pieces of part_steps (the
+ * parts > 1: a key tile's steps - 32 queries of one head each, from the sequence's last back to the first that see it - are walked in up to `parts` pieces of part_steps (the
  * last takes what is left) that meet in a second launch; partial: parts * kv_heads * rows_k * 2 * head_dim floats.
  * Rows outside every sequence are not read and not written.  Non-finite values of a key or value row may reach every query row of its own
  * sequence (also through a probability of zero), never another sequence. */

@@ -55,12 +55,12 @@ def test_parts_cover_the_rows(lq, lk, group, kv, causal):
     p = PackedRows(lq, lk, group=group, causal=causal, device="cpu")
     n, piece = p.parts(kv)
     # the steps of a sequence's first key, seen by all its queries but those that see nothing
-    most = max(-(-(q - max(0, q - k) * causal) // 64) * group for q, k in zip(lq, lk or lq))
+    most = max((-(-q // 32) - max(0, q - k) * causal // 32) * group for q, k in zip(lq, lk or lq))
     assert p.key_most == most
     if n == 1:
-        assert most <= max(16, -(-p.key_work * kv // 512))
+        assert most <= max(32, -(-p.key_work * kv // 512))
     else:
-        assert piece >= 16 and n * piece >= most > (n - 1) * piece
+        assert piece >= 32 and n * piece >= most > (n - 1) * piece
 
 
 @pytest.mark.parametrize("make,error", [
