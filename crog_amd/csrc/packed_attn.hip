@@ -145,6 +145,19 @@ __device__ inline void mma_cols(f32x16* out, const T* tile, int at, int tile_row
   }
 }
 
+// the transposed operands of 16 tile rows from tile_row on, for all column blocks
+template <typename T, int DP>
+__device__ inline void load_cols(bf16x8* v, const T* tile, int at, int tile_row) {
+  using L = Tile<T, DP>;
+#pragma unroll
+  for (int c = 0; c < L::NC; c++) {
+    const char* base = (const char*)tile + tile_row * L::RB;
+    const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(base + (at ^ (c << 6))));
+    const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds_bf16x4*)(base + 8 * L::RB + (at ^ (c << 6) ^ 32)));
+    v[c] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
 // a lane's row of a resident operand, zeros behind the head dimension
 template <typename T, int DP>
 __device__ inline void load_frag(Vec16<T>* frag, const T* row, int h, int dim, bool valid) {
@@ -314,12 +327,46 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
 #pragma unroll
           for (int i = 0; i < 16; i++) o[c][i] *= alpha;
       }
+      if constexpr (sizeof(T) == 2) {
+        // 16 keys a group: the products of a group run while the next one's exponentials are formed
+        constexpr int G = 2 * NB;
+        bf16x8 v[2][L::NC], pb[2];
+        const auto probs = [&](int g) {
 #pragma unroll
-      for (int n = 0; n < NB; n++) {
+          for (int j = 0; j < 8; j++) {
+            const float x = ex2(s[g / 2][8 * (g & 1) + j] * c2 - mu);
+            l += x;
+            pb[g & 1][j] = (bf16)x;
+          }
+        };
+        load_cols<T, DP>(v[0], sV[0], at_c, 0);
+        probs(0);
 #pragma unroll
-        for (int i = 0; i < 16; i++) { s[n][i] = ex2(s[n][i] * c2 - mu); l += s[n][i]; }
+        for (int g = 0; g < G; g++) {
+          if (g + 1 < G) load_cols<T, DP>(v[(g + 1) & 1], sV[0], at_c, (g + 1) * 16);
+#pragma unroll
+          for (int c = 0; c < L::NC; c++) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[g & 1][c], pb[g & 1], o[c], 0, 0, 0);
+          if (g + 1 < G) probs(g + 1);
+#ifdef SGB
+          if (g + 1 < G) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 2 * L::NC, 0);
+#pragma unroll
+          for (int c = 0; c < L::NC; c++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, 20 / L::NC, 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 8 / L::NC, 0);
+          }
+          }
+#endif
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) { s[n][i] = ex2(s[n][i] * c2 - mu); l += s[n][i]; }
           mma_cols<T, DP>(o, sV[0], at_c, n * 32, s[n]);
         }
+      }
     }
     wait_vmcnt<0>();
     __syncthreads();
