@@ -8,9 +8,9 @@
 //   dpre_w = sum dh U, dpre_b = sum dh, dgate = sum dU z, dpost_w = gate sum dU Y, dpost_b = gate sum dU   - sums over the rows
 // so four column sums (dU Y, dU, dh U, dh) give all five.
 //
-// Bound: memory.  Forward reads x, y and writes u, h; backward reads x, y, du, dh and writes dx, dy; the weights stay in registers while a group
-// of TPR threads walks over rows.  A thread holds at most 16 columns (four sums and four weights each are 128 registers): a row takes 16, 64,
-// 256 or 512 threads.  Column sums: registers, then the block's groups through LDS, then one slab row per block, added up in block order by a
+// Bound: memory.  Forward reads x, y and writes u, h (the next row is fetched during this one: 77 -> 46 us at 32768 x 1024 bf16, 268 MB, 5.8 TB/s);
+// backward reads x, y, du, dh and writes dx, dy (403 MB, 90 us, 4.5 TB/s).  The weights stay in registers while a group of TPR threads walks over
+// rows.  A thread holds at most 16 columns (four sums and four weights each are 128 registers): a row takes 16, 64, 256 or 512 threads.  Column sums: registers, then the block's groups through LDS, then one slab row per block, added up in block order by a
 // second launch - no atomics, the same bits every time.
 #include "common.h"
 
@@ -27,27 +27,31 @@ struct GnArgs {
   float alpha, eps;
 };
 
-// VEC consecutive elements; rows of any length and alignment: whole vectors where they are 16-byte aligned, element by element at the ragged end
-template <typename T>
-__device__ inline void load_vec(float* f, const T* row, int c0, int cols, bool aligned) {
+// Rows whose length is a whole number of 16-byte vectors and whose tensors are 16-byte aligned (WHOLE) are read vector by vector, and a thread's
+// vector is there or it is not; other rows element by element.
+template <typename T, bool WHOLE>
+__device__ inline Vec16<T> load_vec(const T* row, int c0, int cols) {
   constexpr int V = Elem<T>::VEC;
-  if (aligned && c0 + V <= cols) {
-    const Vec16<T> v = ldg16(row + c0);
-#pragma unroll
-    for (int e = 0; e < V; e++) f[e] = Elem<T>::to_f(v.v[e]);
+  Vec16<T> v = zero16<T>();
+  if constexpr (WHOLE) {
+    f32x4 q = {0.f, 0.f, 0.f, 0.f};
+    if (c0 < cols) q = *reinterpret_cast<const f32x4*>(row + c0);
+    v = __builtin_bit_cast(Vec16<T>, q);
   } else {
 #pragma unroll
-    for (int e = 0; e < V; e++) f[e] = c0 + e < cols ? Elem<T>::to_f(row[c0 + e]) : 0.f;
+    for (int e = 0; e < V; e++)
+      if (c0 + e < cols) v.v[e] = row[c0 + e];
   }
+  return v;
 }
-template <typename T>
-__device__ inline void store_vec(T* row, const float* f, int c0, int cols, bool aligned) {
+template <typename T, bool WHOLE>
+__device__ inline void store_vec(T* row, const float* f, int c0, int cols) {
   constexpr int V = Elem<T>::VEC;
-  if (aligned && c0 + V <= cols) {
+  if constexpr (WHOLE) {
     Vec16<T> v;
 #pragma unroll
     for (int e = 0; e < V; e++) v.v[e] = Elem<T>::from_f(f[e]);
-    stg16(row + c0, v);
+    if (c0 < cols) stg16(row + c0, v);
   } else {
 #pragma unroll
     for (int e = 0; e < V; e++)
@@ -55,54 +59,67 @@ __device__ inline void store_vec(T* row, const float* f, int c0, int cols, bool 
   }
 }
 
-// sum over the TPR threads of a row, in all of them.  TPR > 64: through LDS (`red`: a slot per wave; the two barriers make it free again)
+// sum over the TPR threads of a row, in all of them.  TPR > 64: through LDS, a slot per wave; two sets in turn, so that one barrier a sum is enough
+// (a set is written again only behind the barrier of the sum between)
+struct Meet {
+  float* slots;      // [2][waves of the block]
+  int turn;
+};
 template <int TPR>
-__device__ inline float row_sum(float v, float* red) {
+__device__ inline float row_sum(float v, Meet& m) {
   if constexpr (TPR <= 64) {
     return group_sum<TPR>(v);
   } else {
+    float* set = m.slots + m.turn * (blockDim.x >> 6);
+    m.turn ^= 1;
     v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) set[threadIdx.x >> 6] = v;
     __syncthreads();
+    const int first = threadIdx.x / TPR * (TPR / 64);
     float t = 0.f;
 #pragma unroll
-    for (int w = 0; w < TPR / 64; w++) t += red[w];
-    __syncthreads();
+    for (int w = 0; w < TPR / 64; w++) t += set[first + w];
     return t;
   }
 }
 
-template <typename T, int TPR, int NV> struct Threads {
+template <typename T, int TPR, int NV, bool WHOLE> struct Threads {
   static constexpr int V = Elem<T>::VEC, N = NV * V;
   static constexpr int THREADS = TPR > 256 ? TPR : 256, GROUPS = THREADS / TPR;
-  // column of element i of the thread
+  // column of element i of thread t, and whether the row has it
   __device__ static inline int col(int t, int i) { return (i / V * TPR + t) * V + i % V; }
+  __device__ static inline bool has(int t, int i, int cols) { return col(t, WHOLE ? i / V * V : i) < cols; }
 };
 
-template <typename T, int TPR, int N>
-__device__ inline void load_row(float (&f)[N], const void* base, long ld, int row, int t, int cols, bool aligned) {
+template <typename T, int NV> struct Row { Vec16<T> v[NV]; };      // a thread's share of a row as it is stored
+template <typename T, int TPR, int NV, bool WHOLE>
+__device__ inline Row<T, NV> fetch(const void* base, long ld, int row, int t, int cols) {
+  Row<T, NV> r;
   const T* p = (const T*)base + (long)row * ld;
 #pragma unroll
-  for (int k = 0; k < N / Elem<T>::VEC; k++) load_vec<T>(f + k * Elem<T>::VEC, p, (k * TPR + t) * Elem<T>::VEC, cols, aligned);
+  for (int k = 0; k < NV; k++) r.v[k] = load_vec<T, WHOLE>(p, (k * TPR + t) * Elem<T>::VEC, cols);
+  return r;
 }
-template <typename T, int TPR, int N>
-__device__ inline void store_row(void* base, long ld, int row, const float (&f)[N], int t, int cols, bool aligned) {
+template <typename T, int NV, int N>
+__device__ inline void widen(float (&f)[N], const Row<T, NV>& r) {
+#pragma unroll
+  for (int i = 0; i < N; i++) f[i] = Elem<T>::to_f(r.v[i / Elem<T>::VEC].v[i % Elem<T>::VEC]);
+}
+template <typename T, int TPR, bool WHOLE, int N>
+__device__ inline void store_row(void* base, long ld, int row, const float (&f)[N], int t, int cols) {
   T* p = (T*)base + (long)row * ld;
 #pragma unroll
-  for (int k = 0; k < N / Elem<T>::VEC; k++) store_vec<T>(p, f + k * Elem<T>::VEC, (k * TPR + t) * Elem<T>::VEC, cols, aligned);
+  for (int k = 0; k < N / Elem<T>::VEC; k++) store_vec<T, WHOLE>(p, f + k * Elem<T>::VEC, (k * TPR + t) * Elem<T>::VEC, cols);
 }
 template <typename S, int N>
-__device__ inline void load_weights(float (&f)[N], const float* w, float otherwise, int t, int cols) {
+__device__ inline void load_weights(float (&f)[N], const float* w, float otherwise, int t, int cols) {      // (0 behind the row's end)
 #pragma unroll
-  for (int i = 0; i < N; i++) {
-    const int c = S::col(t, i);
-    f[i] = w && c < cols ? w[c] : otherwise;
-  }
+  for (int i = 0; i < N; i++) f[i] = S::has(t, i, cols) ? (w ? w[S::col(t, i)] : otherwise) : 0.f;
 }
 
 // f becomes the normalised row; mean and 1 / deviation in two passes over the registers (columns behind the row's end count as nothing)
 template <int TPR, typename S, int N>
-__device__ inline void normalise(float (&f)[N], int t, int cols, bool rms, float eps, float& mean, float& inv, float* red) {
+__device__ inline void normalise(float (&f)[N], int t, int cols, bool rms, float eps, float& mean, float& inv, Meet& red) {
   mean = 0.f;
   if (!rms) {
     float s = 0.f;
@@ -110,7 +127,7 @@ __device__ inline void normalise(float (&f)[N], int t, int cols, bool rms, float
     for (int i = 0; i < N; i++) s += f[i];
     mean = row_sum<TPR>(s, red) / (float)cols;
 #pragma unroll
-    for (int i = 0; i < N; i++) f[i] = S::col(t, i) < cols ? f[i] - mean : 0.f;
+    for (int i = 0; i < N; i++) f[i] = S::has(t, i, cols) ? f[i] - mean : 0.f;
   }
   float q = 0.f;
 #pragma unroll
@@ -120,12 +137,12 @@ __device__ inline void normalise(float (&f)[N], int t, int cols, bool rms, float
   for (int i = 0; i < N; i++) f[i] *= inv;
 }
 
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_fwd_kernel(const GnArgs a, int vec16) {
-  using S = Threads<T, TPR, NV>;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+template <typename T, int TPR, int NV, bool WHOLE>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_fwd_kernel(const GnArgs a) {
+  using S = Threads<T, TPR, NV, WHOLE>;
+  __shared__ float slots[S::THREADS / 32];
+  Meet red{slots, 0};
   const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-  const bool al = vec16;
   float gate[S::N], w1[S::N], b1[S::N], w2[S::N], b2[S::N];
   load_weights<S>(gate, a.gate, 1.f, t, a.cols);
   if (a.has_post) {
@@ -137,12 +154,18 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_fwd_kernel(c
     load_weights<S>(b2, a.pre_b, 0.f, t, a.cols);
   }
   // (a group whose row lies behind the last one joins the cross-lane sums with the last row's values and stores nothing)
-  for (int base = blockIdx.x * S::GROUPS; base < a.rows; base += gridDim.x * S::GROUPS) {
-    const int row = base + grp, rc = min(row, a.rows - 1);
+  const int step = gridDim.x * S::GROUPS;
+  int row = blockIdx.x * S::GROUPS + grp;
+  Row<T, NV> nx = fetch<T, TPR, NV, WHOLE>(a.x, a.ldx, min(row, a.rows - 1), t, a.cols), ny = fetch<T, TPR, NV, WHOLE>(a.y, a.ldy, min(row, a.rows - 1), t, a.cols);
+  for (int base = blockIdx.x * S::GROUPS; base < a.rows; base += step, row += step) {
     const bool live = row < a.rows;
     float x[S::N], y[S::N];
-    load_row<T, TPR>(x, a.x, a.ldx, rc, t, a.cols, al);
-    load_row<T, TPR>(y, a.y, a.ldy, rc, t, a.cols, al);
+    widen(x, nx);
+    widen(y, ny);
+    if (base + step < a.rows) {      // the next row is on its way during this one
+      nx = fetch<T, TPR, NV, WHOLE>(a.x, a.ldx, min(row + step, a.rows - 1), t, a.cols);
+      ny = fetch<T, TPR, NV, WHOLE>(a.y, a.ldy, min(row + step, a.rows - 1), t, a.cols);
+    }
     float mean1 = 0.f, inv1 = 1.f, mean2 = 0.f, inv2 = 1.f;
     if (a.has_post) {
       normalise<TPR, S>(y, t, a.cols, a.rms, a.eps, mean1, inv1, red);
@@ -150,36 +173,36 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_fwd_kernel(c
       for (int i = 0; i < S::N; i++) y[i] = y[i] * w1[i] + b1[i];
     }
 #pragma unroll
-    for (int i = 0; i < S::N; i++) x[i] = S::col(t, i) < a.cols ? a.alpha * x[i] + gate[i] * y[i] : 0.f;
-    if (live) store_row<T, TPR>(a.u, a.ldu, row, x, t, a.cols, al);
+    for (int i = 0; i < S::N; i++) x[i] = a.alpha * x[i] + gate[i] * y[i];
+    if (live) store_row<T, TPR, WHOLE>(a.u, a.ldu, row, x, t, a.cols);
     if (a.has_pre) {
       normalise<TPR, S>(x, t, a.cols, a.rms, a.eps, mean2, inv2, red);
 #pragma unroll
       for (int i = 0; i < S::N; i++) x[i] = x[i] * w2[i] + b2[i];
-      if (live) store_row<T, TPR>(a.h, a.ldh, row, x, t, a.cols, al);
+      if (live) store_row<T, TPR, WHOLE>(a.h, a.ldh, row, x, t, a.cols);
     }
     if (a.stats && live && t == 0) *reinterpret_cast<f32x4*>(a.stats + 4 * (long)row) = f32x4{mean1, inv1, mean2, inv2};
   }
 }
 
 // d becomes N'(d) for the normalised row n
-template <int TPR, int N>
-__device__ inline void normalise_back(float (&d)[N], const float (&n)[N], int cols, bool rms, float inv, float* red) {
+template <int TPR, typename S, int N>
+__device__ inline void normalise_back(float (&d)[N], const float (&n)[N], int t, int cols, bool rms, float inv, Meet& red) {
   float s = 0.f, q = 0.f;
 #pragma unroll
   for (int i = 0; i < N; i++) { s += d[i]; q += d[i] * n[i]; }
   const float md = rms ? 0.f : row_sum<TPR>(s, red) / (float)cols, mq = row_sum<TPR>(q, red) / (float)cols;
 #pragma unroll
-  for (int i = 0; i < N; i++) d[i] = (d[i] - md - n[i] * mq) * inv;
+  for (int i = 0; i < N; i++) d[i] = S::has(t, i, cols) ? (d[i] - md - n[i] * mq) * inv : 0.f;
 }
 
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_bwd_kernel(const GnArgs a, int vec16) {
-  using S = Threads<T, TPR, NV>;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+template <typename T, int TPR, int NV, bool WHOLE>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_bwd_kernel(const GnArgs a) {
+  using S = Threads<T, TPR, NV, WHOLE>;
+  __shared__ float slots[S::THREADS / 32];
+  Meet red{slots, 0};
   __shared__ float part[S::GROUPS > 1 ? S::THREADS : 1];
   const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-  const bool al = vec16;
   float gate[S::N], w1[S::N], b1[S::N], w2[S::N];
   load_weights<S>(gate, a.gate, 1.f, t, a.cols);
   load_weights<S>(w1, a.post_w, 1.f, t, a.cols);
@@ -192,45 +215,52 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_bwd_kernel(c
     for (int i = 0; i < S::N; i++) sum[k][i] = 0.f;
   for (int base = blockIdx.x * S::GROUPS; base < a.rows; base += gridDim.x * S::GROUPS) {
     const int row = base + grp, rc = min(row, a.rows - 1);
-    const bool live = row < a.rows;
+    const bool live = row < a.rows, both = a.has_pre && a.dh;
     const f32x4 st = *reinterpret_cast<const f32x4*>(a.stats + 4 * (long)rc);
-    float y[S::N], d[S::N];      // Y (y itself without a post norm), dU
-    load_row<T, TPR>(y, a.y, a.ldy, rc, t, a.cols, al);
-#pragma unroll
-    for (int i = 0; i < S::N; i++) {
-      y[i] = (a.has_post && S::col(t, i) < a.cols) ? (y[i] - st[0]) * st[1] : y[i];
-      d[i] = 0.f;
+    const Row<T, NV> ry = fetch<T, TPR, NV, WHOLE>(a.y, a.ldy, rc, t, a.cols);
+    Row<T, NV> rx{}, rh{}, ru{};
+    if (both) {
+      rx = fetch<T, TPR, NV, WHOLE>(a.x, a.ldx, rc, t, a.cols);
+      rh = fetch<T, TPR, NV, WHOLE>(a.dh, a.lddh, rc, t, a.cols);
     }
-    if (a.has_pre && a.dh) {
+    if (a.du) ru = fetch<T, TPR, NV, WHOLE>(a.du, a.lddu, rc, t, a.cols);
+    float y[S::N], d[S::N];      // Y (y itself without a post norm), dU
+    widen(y, ry);
+    if (a.has_post)
+#pragma unroll
+      for (int i = 0; i < S::N; i++) y[i] = S::has(t, i, a.cols) ? (y[i] - st[0]) * st[1] : 0.f;
+    if (both) {
       float u[S::N], g[S::N];
-      load_row<T, TPR>(u, a.x, a.ldx, rc, t, a.cols, al);
-      load_row<T, TPR>(g, a.dh, a.lddh, rc, t, a.cols, al);
+      widen(u, rx);
+      widen(g, rh);
 #pragma unroll
       for (int i = 0; i < S::N; i++) {
         const float z = a.has_post ? y[i] * w1[i] + b1[i] : y[i];
-        u[i] = S::col(t, i) < a.cols ? (a.alpha * u[i] + gate[i] * z - st[2]) * st[3] : 0.f;
+        u[i] = S::has(t, i, a.cols) ? (a.alpha * u[i] + gate[i] * z - st[2]) * st[3] : 0.f;
         if (live) { sum[2][i] += g[i] * u[i]; sum[3][i] += g[i]; }
         d[i] = g[i] * w2[i];
       }
-      normalise_back<TPR>(d, u, a.cols, a.rms, st[3], red);
+      normalise_back<TPR, S>(d, u, t, a.cols, a.rms, st[3], red);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::N; i++) d[i] = 0.f;
     }
     if (a.du) {
       float g[S::N];
-      load_row<T, TPR>(g, a.du, a.lddu, rc, t, a.cols, al);
+      widen(g, ru);
 #pragma unroll
       for (int i = 0; i < S::N; i++) d[i] += g[i];
     }
     float o[S::N];
 #pragma unroll
     for (int i = 0; i < S::N; i++) {
-      if (S::col(t, i) >= a.cols) d[i] = 0.f;
       if (live) { sum[0][i] += d[i] * y[i]; sum[1][i] += d[i]; }
       o[i] = a.alpha * d[i];
-      d[i] = d[i] * gate[i] * (a.has_post ? w1[i] : 1.f);
+      d[i] = a.has_post ? d[i] * gate[i] * w1[i] : d[i] * gate[i];
     }
-    if (live && a.dx) store_row<T, TPR>(a.dx, a.lddx, row, o, t, a.cols, al);
-    if (a.has_post) normalise_back<TPR>(d, y, a.cols, a.rms, st[1], red);
-    if (live && a.dy) store_row<T, TPR>(a.dy, a.lddy, row, d, t, a.cols, al);
+    if (live && a.dx) store_row<T, TPR, WHOLE>(a.dx, a.lddx, row, o, t, a.cols);
+    if (a.has_post) normalise_back<TPR, S>(d, y, t, a.cols, a.rms, st[1], red);
+    if (live && a.dy) store_row<T, TPR, WHOLE>(a.dy, a.lddy, row, d, t, a.cols);
   }
   if (!a.slab) return;
 #pragma unroll
@@ -252,27 +282,35 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_bwd_kernel(c
     }
 }
 
-// the blocks' sums in order -> the five gradients, added onto what the buffers hold.  A block takes 16 columns, 16 runs of slab rows each.
-__global__ void __launch_bounds__(256) gated_norm_sums_kernel(const float* slab, int blocks, int cols, const float* gate, const float* post_w,
-                                                              const float* post_b, int has_post, float* dgate, float* dpost_w, float* dpost_b,
-                                                              float* dpre_w, float* dpre_b) {
-  __shared__ float part[4][16][17];
+// the blocks' sums in order -> the five gradients, added onto what the buffers hold.  A block takes 16 columns, 64 runs of slab rows each (latency: 512
+// slab rows of 1024 columns are 8 MB, 64 blocks; 16 runs took 13.9 us)
+constexpr int RUNS = 64;
+__global__ void __launch_bounds__(16 * RUNS) gated_norm_sums_kernel(const float* slab, int blocks, int cols, const float* gate, const float* post_w,
+                                                                    const float* post_b, int has_post, float* dgate, float* dpost_w, float* dpost_b,
+                                                                    float* dpre_w, float* dpre_b) {
+  __shared__ float part[4][RUNS][17];
   const int c = blockIdx.x * 16 + (threadIdx.x & 15), run = threadIdx.x >> 4;
-  const int per = (blocks + 15) / 16, lo = run * per, hi = min(lo + per, blocks);
+  const int per = (blocks + RUNS - 1) / RUNS, lo = run * per, hi = min(lo + per, blocks);
   float s[4] = {0.f, 0.f, 0.f, 0.f};
   if (c < cols)
+#pragma unroll 4
     for (int b = lo; b < hi; b++)
 #pragma unroll
       for (int k = 0; k < 4; k++) s[k] += slab[((long)b * 4 + k) * cols + c];
 #pragma unroll
   for (int k = 0; k < 4; k++) part[k][run][threadIdx.x & 15] = s[k];
   __syncthreads();
+  __shared__ float total[4][16];
+  if (run < 4) {      // (run = which of the four sums)
+    float t = 0.f;
+#pragma unroll
+    for (int r = 0; r < RUNS; r++) t += part[run][r][threadIdx.x & 15];
+    total[run][threadIdx.x & 15] = t;
+  }
+  __syncthreads();
   if (run != 0 || c >= cols) return;
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    s[k] = 0.f;
-    for (int r = 0; r < 16; r++) s[k] += part[k][r][threadIdx.x];
-  }
+  for (int k = 0; k < 4; k++) s[k] = total[k][threadIdx.x];
   const float g = gate ? gate[c] : 1.f;
   if (dgate) dgate[c] += has_post ? (post_w ? post_w[c] : 1.f) * s[0] + (post_b ? post_b[c] : 0.f) * s[1] : s[0];
   if (dpost_w) dpost_w[c] += g * s[0];
@@ -282,9 +320,9 @@ __global__ void __launch_bounds__(256) gated_norm_sums_kernel(const float* slab,
 }
 
 constexpr int MAX_COLS = 8192;
-constexpr int MAX_BLOCKS = 512;      // two per CU
+constexpr int MAX_BLOCKS = 512;      // two per CU.  (32768 x 1024 bf16: forward 46.0 us, with 1024 / 2048 blocks 53.7 / 49.2; backward 89.6, with 768 105)
 
-// threads of a row: 16 columns a thread at most
+// threads of a row: 16 columns a thread at most.  (8 a thread, a row of 1024 columns on two waves that meet in LDS: 55.6 / 122 us)
 int threads_per_row(int cols) { return cols <= 256 ? 16 : cols <= 1024 ? 64 : cols <= 4096 ? 256 : 512; }
 int blocks_for(int rows, int cols) {
   const int tpr = threads_per_row(cols), groups = tpr > 256 ? 1 : 256 / tpr;
@@ -292,31 +330,29 @@ int blocks_for(int rows, int cols) {
   return n < MAX_BLOCKS ? n : MAX_BLOCKS;
 }
 
-template <typename T, int TPR, int NV>
-void launch(const GnArgs& a, bool fwd, int vec16, int blocks, hipStream_t s) {
-  if (fwd) gated_norm_fwd_kernel<T, TPR, NV><<<blocks, Threads<T, TPR, NV>::THREADS, 0, s>>>(a, vec16);
-  else gated_norm_bwd_kernel<T, TPR, NV><<<blocks, Threads<T, TPR, NV>::THREADS, 0, s>>>(a, vec16);
+template <typename T, int TPR, int NV, bool WHOLE>
+void launch(const GnArgs& a, bool fwd, hipStream_t s) {
+  const int blocks = blocks_for(a.rows, a.cols);
+  if (fwd) gated_norm_fwd_kernel<T, TPR, NV, WHOLE><<<blocks, Threads<T, TPR, NV, WHOLE>::THREADS, 0, s>>>(a);
+  else gated_norm_bwd_kernel<T, TPR, NV, WHOLE><<<blocks, Threads<T, TPR, NV, WHOLE>::THREADS, 0, s>>>(a);
 }
 template <typename T, int TPR>
-void launch_nv(const GnArgs& a, bool fwd, int vec16, int blocks, hipStream_t s) {
-  const int nv = cdiv(a.cols, TPR * Elem<T>::VEC);      // (at most 16 columns a thread: threads_per_row)
-  if constexpr (sizeof(T) == 2) {
-    if (nv == 1) launch<T, TPR, 1>(a, fwd, vec16, blocks, s);
-    else launch<T, TPR, 2>(a, fwd, vec16, blocks, s);
-  } else {
-    if (nv == 1) launch<T, TPR, 1>(a, fwd, vec16, blocks, s);
-    else if (nv == 2) launch<T, TPR, 2>(a, fwd, vec16, blocks, s);
-    else launch<T, TPR, 4>(a, fwd, vec16, blocks, s);
-  }
+void launch_nv(const GnArgs& a, bool fwd, bool whole, hipStream_t s) {
+  constexpr int MOST = 16 / Elem<T>::VEC;                // 16 columns a thread at most (threads_per_row)
+  const int nv = cdiv(a.cols, TPR * Elem<T>::VEC);
+  if (!whole) launch<T, TPR, MOST, false>(a, fwd, s);
+  else if (nv == 1) launch<T, TPR, 1, true>(a, fwd, s);
+  else if (nv == 2 || MOST == 2) launch<T, TPR, 2, true>(a, fwd, s);
+  else launch<T, TPR, MOST, true>(a, fwd, s);
 }
 template <typename T>
-void launch_t(const GnArgs& a, bool fwd, int vec16, hipStream_t s) {
-  const int blocks = blocks_for(a.rows, a.cols);
+void launch_t(const GnArgs& a, bool fwd, bool aligned, hipStream_t s) {
+  const bool whole = aligned && a.cols % Elem<T>::VEC == 0;
   switch (threads_per_row(a.cols)) {
-    case 16: launch_nv<T, 16>(a, fwd, vec16, blocks, s); break;
-    case 64: launch_nv<T, 64>(a, fwd, vec16, blocks, s); break;
-    case 256: launch_nv<T, 256>(a, fwd, vec16, blocks, s); break;
-    default: launch_nv<T, 512>(a, fwd, vec16, blocks, s); break;
+    case 16: launch_nv<T, 16>(a, fwd, whole, s); break;
+    case 64: launch_nv<T, 64>(a, fwd, whole, s); break;
+    case 256: launch_nv<T, 256>(a, fwd, whole, s); break;
+    default: launch_nv<T, 512>(a, fwd, whole, s); break;
   }
 }
 
@@ -369,7 +405,7 @@ extern "C" int crog_gated_norm_bwd(int dtype, const void* x, int64_t ldx, const 
   else launch_t<float>(a, false, vec16, (hipStream_t)stream);
   CROG_LAUNCH_CHECK();
   if (sums) {
-    gated_norm_sums_kernel<<<cdiv(cols, 16), 256, 0, (hipStream_t)stream>>>(slab, blocks_for(rows, cols), cols, gate, post_w, post_b, has_post, dgate, dpost_w,
+    gated_norm_sums_kernel<<<cdiv(cols, 16), 16 * RUNS, 0, (hipStream_t)stream>>>(slab, blocks_for(rows, cols), cols, gate, post_w, post_b, has_post, dgate, dpost_w,
                                                                             dpost_b, dpre_w, dpre_b);
     CROG_LAUNCH_CHECK();
   }
