@@ -1245,6 +1245,19 @@ def mha(xq, xk, xv, wq: WRef, wk: WRef, wv: WRef, bq, bk, bv, wo: WRef, bo, *, B
 # ------------------------------------------------------------------------------------------------
 # a transformer block on packed rows: attention, rotary positions, the gated residual between two norms
 # ------------------------------------------------------------------------------------------------
+def _first_order(backward):
+    """once_differentiable, whose bookkeeping costs as much as a small launch, only where a graph of the backward pass is asked for."""
+    recorded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
+def _fresh(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 class PackedAttentionFn(Function):
     """o = softmax(scale q k^T) v within each sequence of a PackedRows plan (the packed form of the attention inside MhaFn: clip.py:246-260,
     layers.py:291-296,329-332), any head dim up to 128, grouped key heads."""
@@ -1254,7 +1267,7 @@ class PackedAttentionFn(Function):
         ctx.set_materialize_grads(False)
         ctx.shapes = (q.shape, k.shape, v.shape)
         empty = rows.rows_q == 0 or rows.rows_k == 0
-        o = (torch.zeros if empty else torch.empty)(q.shape, device=q.device, dtype=q.dtype)
+        o = torch.zeros(q.shape, device=q.device, dtype=q.dtype) if empty else _fresh(q)
         lse = None
         if not empty:
             q, k, v = K.heads16(q), K.heads16(k), K.heads16(v)
@@ -1268,7 +1281,7 @@ class PackedAttentionFn(Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, do):
         if do is None:
             return (None,) * 5
@@ -1277,7 +1290,7 @@ class PackedAttentionFn(Function):
             return tuple(torch.zeros(s, device=do.device, dtype=do.dtype) for s in ctx.shapes) + (None, None)
         q, k, v, o, lse = ctx.saved_tensors
         do = K.heads16(do)
-        dq, dk, dv = (torch.empty(s, device=q.device, dtype=q.dtype) for s in ctx.shapes)
+        dq, dk, dv = _fresh(q), _fresh(k), _fresh(v)
         K.packed_attn_bwd(q, k, v, o, do, lse, torch.empty_like(lse), dq, dk, dv, rows, scale)
         for t, n in ((dq, rows.rows_q), (dk, rows.rows_k), (dv, rows.rows_k)):
             if t.shape[0] > n:
@@ -1320,13 +1333,13 @@ class RotaryFn(Function):
     @staticmethod
     def _turn(q, k, positions, axes, inverse):
         q, k = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (q, k))
-        qo, ko = (None if t is None else torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k))
+        qo, ko = (None if t is None else _fresh(t) for t in (q, k))
         if q is not None or k is not None:
             K.rotary(q, k, qo, ko, positions, axes, inverse=inverse)
         return qo, ko
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dq, dk):
         positions, = ctx.saved_tensors
         dq, dk = RotaryFn._turn(dq, dk, positions, ctx.axes, True)
@@ -1355,21 +1368,28 @@ def rotary(q, k, positions, axes):
     return RotaryFn.apply(q, k, positions, axes)
 
 
+def _at(r: Optional[WRef], buf: str):
+    """Address of a weight's values ("P") or of its gradient ("G"); None for no weight (or one that takes no gradient)."""
+    if r is None or (buf == "G" and not r.param.requires_grad):
+        return None
+    return getattr(r.store, buf).data_ptr() + 4 * r.off
+
+
 class GatedNormFn(Function):
     @staticmethod
     def forward(ctx, x, y, gate, post, pre, alpha, eps, rms, *params):
         ctx.set_materialize_grads(False)
-        u = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if pre is not None else None
-        stats = torch.empty(x.numel() // x.shape[-1], 4, device=x.device, dtype=torch.float32) if any(ctx.needs_input_grad) else None
-        masters = [None if w is None else tuple(r.master() if r is not None else None for r in w) for w in (post, pre)]
-        K.gated_norm_fwd(x, y, gate.master() if gate is not None else None, *masters, rms, alpha, eps, u, h, stats)
+        u = _fresh(x)
+        h = _fresh(x) if pre is not None else None
+        stats = x.new_empty((x.numel() // x.shape[-1], 4), dtype=torch.float32) if any(ctx.needs_input_grad) else None
+        weights = [_at(r, "P") for r in (gate, *(post or (None, None)), *(pre or (None, None)))]
+        K.gated_norm_fwd(x, y, weights, post is not None, pre is not None, rms, alpha, eps, u, h, stats)
         ctx.cfg = (gate, post, pre, alpha, rms)
         ctx.save_for_backward(x, y, stats)
         return u, h
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, du, dh):
         gate, post, pre, alpha, rms = ctx.cfg
         x, y, stats = ctx.saved_tensors
@@ -1377,17 +1397,13 @@ class GatedNormFn(Function):
         if du is None and dh is None:
             return (None, None) + none
         du, dh = (K.as_mat(t) if t is not None else None for t in (du, dh))
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
-        dy = torch.empty(x.shape, device=x.device, dtype=x.dtype) if ctx.needs_input_grad[1] else None
-
-        def grad(r):
-            return r.grad() if r is not None and r.param.requires_grad else None
-        masters = [None if w is None else tuple(r.master() if r is not None else None for r in w) for w in (post, pre)]
-        post, pre = post or (None, None), pre or (None, None)
-        K.gated_norm_bwd(x, y, du, dh, gate.master() if gate is not None else None, *masters, rms, alpha, stats, dx, dy, grad(gate),
-                         [grad(r) for r in post], [grad(r) for r in pre])
-        for r in (gate, *post, *pre):
-            if grad(r) is not None:
+        dx = _fresh(x) if ctx.needs_input_grad[0] else None
+        dy = _fresh(y) if ctx.needs_input_grad[1] else None
+        refs = (gate, *(post or (None, None)), *(pre or (None, None)))
+        grads = [_at(r, "G") for r in refs]
+        K.gated_norm_bwd(x, y, du, dh, [_at(r, "P") for r in refs], post is not None, pre is not None, rms, alpha, stats, dx, dy, grads)
+        for r, g in zip(refs, grads):
+            if g is not None:
                 r.done()
         return (dx, dy) + none
 
@@ -1419,7 +1435,7 @@ def gated_norm(x, y, *, post=None, gate: Optional[WRef] = None, pre=None, res_sc
             raise ValueError(f"gated_norm: a weight of {r.rows * r.cols} values for rows of {C} columns")
     if not eps >= 0 or not math.isfinite(res_scale):
         raise ValueError("gated_norm: eps must not be negative and res_scale must be finite")
-    K.same_device(x, y, *[r.P for r in refs])
+    K.same_device(x, y, *{id(r.P): r.P for r in refs}.values())
     return GatedNormFn.apply(K.as_mat(x), K.as_mat(y), gate, post, pre, float(res_scale), float(eps), bool(rms), *[r.param for r in refs])
 
 

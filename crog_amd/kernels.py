@@ -803,27 +803,21 @@ def rotary(q, k, q_out, k_out, positions, axes, inverse=False):
                             0 if k is None else k.shape[1], t.shape[2], axes.pairs, axes.axes, axes.interleaved, int(inverse), stream()), "rotary")
 
 
-def gated_norm_fwd(x, y, gate, post, pre, rms, alpha, eps, u, h, stats):
-    """post / pre: None or (weight or None, bias or None), fp32 [C]; h None without a pre norm."""
+def gated_norm_fwd(x, y, weights, has_post, has_pre, rms, alpha, eps, u, h, stats):
+    """weights: addresses of gate, post weight, post bias, pre weight, pre bias (fp32 [C]; None = 1 or 0).  h None without a pre norm."""
     M, C, ldx = mat(x)
-    pw, pb = post if post is not None else (None, None)
-    nw, nb = pre if pre is not None else (None, None)
-    check(lib().crog_gated_norm_fwd(dcode(x), x.data_ptr(), ldx, y.data_ptr(), mat(y)[2], ptr(gate), ptr(pw), ptr(pb), ptr(nw), ptr(nb),
-                                    int(post is not None), int(pre is not None), int(rms), float(alpha), float(eps), M, C, u.data_ptr(), mat(u)[2],
-                                    ptr(h), mat(h)[2] if h is not None else 0, ptr(stats), stream()), "gated_norm_fwd")
+    check(lib().crog_gated_norm_fwd(dcode(x), x.data_ptr(), ldx, y.data_ptr(), mat(y)[2], *weights, has_post, has_pre, rms, alpha, eps, M, C, u.data_ptr(),
+                                    C, ptr(h), C, ptr(stats), stream()), "gated_norm_fwd")
 
 
-def gated_norm_bwd(x, y, du, dh, gate, post, pre, rms, alpha, stats, dx, dy, dgate, dpost, dpre):
-    """dpost / dpre: (weight gradient or None, bias gradient or None), added onto."""
+def gated_norm_bwd(x, y, du, dh, weights, has_post, has_pre, rms, alpha, stats, dx, dy, grads):
+    """grads: addresses of the weights' gradients in the order of `weights` (None = not wanted), added onto."""
     M, C, ldx = mat(x)
-    pw, pb = post if post is not None else (None, None)
-    sums = [dgate, *dpost, *dpre]
     slab = None
-    if any(t is not None for t in sums):
+    if any(g is not None for g in grads):
         slab = torch.empty(lib().crog_gated_norm_slab_floats(M, C), device=x.device, dtype=torch.float32)
 
     def two(t):
         return (None, 0) if t is None else (t.data_ptr(), mat(t)[2])
-    check(lib().crog_gated_norm_bwd(dcode(x), x.data_ptr(), ldx, y.data_ptr(), mat(y)[2], *two(du), *two(dh), ptr(gate), ptr(pw), ptr(pb),
-                                    ptr(pre[0]) if pre is not None else None, int(post is not None), int(pre is not None), int(rms), float(alpha), M, C,
-                                    ptr(stats), *two(dx), *two(dy), ptr(slab), *[ptr(t) for t in sums], stream()), "gated_norm_bwd")
+    check(lib().crog_gated_norm_bwd(dcode(x), x.data_ptr(), ldx, y.data_ptr(), mat(y)[2], *two(du), *two(dh), *weights[:4], has_post, has_pre, rms, alpha, M, C,
+                                    ptr(stats), *two(dx), *two(dy), ptr(slab), *grads, stream()), "gated_norm_bwd")
