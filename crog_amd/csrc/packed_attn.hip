@@ -384,33 +384,76 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
   if (h == 0 && a.lse) a.lse[(long)(kh * a.group + hd) * a.rows_q + e.q0 + qi] = l == 0.f ? INFINITY : m + __log2f(l);
 }
 
-// the splits of a row meet: o = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.  One wave per row.
-template <typename T>
+// the splits of a row meet: o = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.  W waves of a row take every W-th split each (W = 4 from 8 splits on: one
+// row of 63 splits took 21.7 us on one wave); a lane takes the statistics of one of its wave's splits, so that their loads, and after that those of
+// the partial rows, are in flight together.
+template <typename T, int W>
 __global__ void __launch_bounds__(NT) packed_combine_kernel(const PackedArgs a, int splits) {
-  const int lane = threadIdx.x & 63;
-  const long total = (long)a.kv_heads * a.rows_q * a.group, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int ROWS = 4 / W;
+  __shared__ float sm[4], part[4][3][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % W;
+  const long per = (long)a.rows_q * a.group, total = a.kv_heads * per, row = (long)blockIdx.x * ROWS + wave / W;
+  const int kh = (int)(min(row, total - 1) / per);
+  const long rr = min(row, total - 1) - kh * per;
   // rows behind the last sequence have no partial result and stay as they are
-  if (row >= total || (row % ((long)a.rows_q * a.group)) >= (long)min(a.cu_q[a.seqs], a.rows_q) * a.group) return;
-  const int kh = (int)(row / ((long)a.rows_q * a.group));
-  const long rr = row % ((long)a.rows_q * a.group);
-  float M = -INFINITY;
-  for (int z = 0; z < splits; z++) M = fmaxf(M, a.part_ml[2 * (z * total + row)]);
-  float l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int z = 0; z < splits; z++) {
-    const float mz = a.part_ml[2 * (z * total + row)], lz = a.part_ml[2 * (z * total + row) + 1];
-    const float f = mz == -INFINITY ? (lz == 0.f ? 0.f : 1.f) : ex2(mz - M);
-    const float* p = a.part_o + (z * total + row) * a.dim;
-    l += f * lz;
-    if (f != 0.f) {
-      if (lane < a.dim) o0 += f * p[lane];
-      if (lane + 64 < a.dim) o1 += f * p[lane + 64];
+  const bool live = row < total && rr < (long)min(a.cu_q[a.seqs], a.rows_q) * a.group;
+  const auto stat = [&](int z, float& m, float& l) {
+    const float2 v = live && z < splits ? *reinterpret_cast<const float2*>(a.part_ml + 2 * (z * total + row)) : make_float2(-INFINITY, 0.f);
+    m = v.x;
+    l = v.y;
+  };
+  float m, l, M = -INFINITY;
+  for (int z0 = w; z0 < splits; z0 += 64 * W) {
+    stat(z0 + lane * W, m, l);
+    M = fmaxf(M, m);
+  }
+  M = wave_max(M);
+  if constexpr (W > 1) {
+    if (lane == 0) sm[wave] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  }
+  float sum = 0.f, o0 = 0.f, o1 = 0.f;
+  const int c0 = min(lane, a.dim - 1), c1 = min(lane + 64, a.dim - 1);
+  for (int z0 = w; z0 < splits; z0 += 64 * W) {
+    stat(z0 + lane * W, m, l);
+    // (a split without a key: m = -inf, l = 0, o = 0; one whose scores were all NaN: m = -inf, l NaN, which has to come through)
+    const float f = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - M);
+    sum += f * l;
+    const int n = live ? min(64, (splits - z0 + W - 1) / W) : 0;
+    const float* p = a.part_o + (z0 * total + row) * a.dim;
+#pragma unroll 8
+    for (int z = 0; z < n; z++) {
+      const float fz = readlane_f(f, z);
+      o0 += fz * p[z * W * total * a.dim + c0];
+      o1 += fz * p[z * W * total * a.dim + c1];
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  sum = wave_sum(sum);
+  if constexpr (W > 1) {
+    part[wave][0][lane] = sum;
+    part[wave][1][lane] = o0;
+    part[wave][2][lane] = o1;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int k = 1; k < W; k++) {
+      sum += part[k][0][lane];
+      o0 += part[k][1][lane];
+      o1 += part[k][2][lane];
+    }
+  }
+  if (!live) return;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* op = (T*)a.Out + (rr / a.group) * a.ldo + (long)(kh * a.group + rr % a.group) * a.hso;
   if (lane < a.dim) op[lane] = Elem<T>::from_f(o0 * inv);
   if (lane + 64 < a.dim) op[lane + 64] = Elem<T>::from_f(o1 * inv);
-  if (lane == 0 && a.lse) a.lse[(kh * a.group + rr % a.group) * a.rows_q + rr / a.group] = l == 0.f ? INFINITY : M + __log2f(l);
+  if (lane == 0 && a.lse) a.lse[(kh * a.group + rr % a.group) * a.rows_q + rr / a.group] = sum == 0.f ? INFINITY : M + __log2f(sum);
+}
+template <typename T>
+void launch_combine(const PackedArgs& a, int splits, int64_t total, hipStream_t s) {
+  if (splits < 8) packed_combine_kernel<T, 1><<<cdiv(total, 4), NT, 0, s>>>(a, splits);
+  else packed_combine_kernel<T, 4><<<(unsigned)total, NT, 0, s>>>(a, splits);
 }
 
 // =====================================================================================================================
@@ -752,8 +795,8 @@ extern "C" int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64
   }
   CROG_LAUNCH_CHECK();
   if (splits > 1) {
-    if (dtype == CROG_BF16) packed_combine_kernel<bf16><<<cdiv(total, 4), NT, 0, s>>>(a, splits);
-    else packed_combine_kernel<float><<<cdiv(total, 4), NT, 0, s>>>(a, splits);
+    if (dtype == CROG_BF16) launch_combine<bf16>(a, splits, total, s);
+    else launch_combine<float>(a, splits, total, s);
     CROG_LAUNCH_CHECK();
   }
   return CROG_OK;

@@ -98,6 +98,7 @@ CASES = [
     ([40, 50], [3, 20], 4, 1, 64, False),
     ([1, 1, 1], [700, 1, 1300], 2, 4, 128, True),          # single tokens over long keys: the split form
     ([2, 5, 1], [900, 64, 2049], 1, 1, 32, True),
+    ([1, 3], [40000, 6], 1, 2, 64, True),                  # a hundred splits
     ([100, 10, 64], [30, 0, 64], 2, 2, 64, True),          # more queries than keys: rows without a key; no key at all
     ([0, 5], [9, 5], 1, 2, 96, False),
     ([300], [700], 2, 2, 120, True),
