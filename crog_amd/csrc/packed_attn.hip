@@ -12,6 +12,7 @@
 // One LDS image serves both ways of reading a tile - rows (16 bytes a lane, lane = row) and columns (ds_read_b64_tr_b16, four rows x 64 bytes a
 // half wave): the 16-byte slot of a row is XORed with the row's low bits, the lowest two moved to the slot's high bits.
 #include "gemm_dma.h"
+#include <type_traits>
 
 namespace {
 
@@ -73,10 +74,11 @@ __device__ inline unsigned lds_of(const void* p) {      // the LDS byte address 
 }
 __device__ inline void opaque(int& x) { asm volatile("" : "+v"(x)); }      // keeps what is computed from x inside the loop it stands in
 
-template <typename T, int DP> struct Tile {
+// (DP: elements of a row in LDS, 64 or 128; DC <= DP: the columns that enter the products, a multiple of 32)
+template <typename T, int DP, int DC> struct Tile {
   static constexpr int VEC = Elem<T>::VEC, CPR = DP / VEC;      // 16-byte chunks per row
-  static constexpr int NS = CPR / 2;                            // 16-byte operand steps of a lane (its half takes every other chunk)
-  static constexpr int NC = DP / 32;                            // 32-column blocks
+  static constexpr int NS = DC / VEC / 2;                       // 16-byte operand steps of a lane (its half takes every other chunk)
+  static constexpr int NC = DC / 32;                            // 32-column blocks
   __device__ static constexpr int slot(int row) { return CPR == 8 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3)); }
   static constexpr int RB = DP * (int)sizeof(T);      // bytes of a row
   // Byte offsets of a lane in a tile.  Its other operands of the tile differ from these by XORs with constants and by whole rows (an instruction's
@@ -100,9 +102,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 __device__ inline float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // acc (32 rows of the tile x 32 columns = lanes) += tile rows . frag (the lane's row of the other operand).  at: rows_at + the buffer's offset
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 __device__ inline void mma_rows(f32x16& acc, const T* tile, int at, int tile_row, const Vec16<T>* frag) {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, DC>;
 #pragma unroll
   for (int ks = 0; ks < L::NS; ks++) {
     const Vec16<T> a = ldg16((const T*)((const char*)tile + (at ^ (ks << 5)) + tile_row * L::RB));
@@ -116,9 +118,9 @@ __device__ inline void mma_rows(f32x16& acc, const T* tile, int at, int tile_row
 }
 
 // out[c] (columns 32 c .. 32 c + 31 of the tile x lanes) += tile^T . p, p = 32 tile rows (registers, acc_row order) x lanes.  at: cols_at + ...
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 __device__ inline void mma_cols(f32x16* out, const T* tile, int at, int tile_row, const f32x16& p) {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, DC>;
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int t = 0; t < 2; t++) {
@@ -146,9 +148,9 @@ __device__ inline void mma_cols(f32x16* out, const T* tile, int at, int tile_row
 }
 
 // the transposed operands of 16 tile rows from tile_row on, for all column blocks
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 __device__ inline void load_cols(bf16x8* v, const T* tile, int at, int tile_row) {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, DC>;
 #pragma unroll
   for (int c = 0; c < L::NC; c++) {
     const char* base = (const char*)tile + tile_row * L::RB;
@@ -159,9 +161,9 @@ __device__ inline void load_cols(bf16x8* v, const T* tile, int at, int tile_row)
 }
 
 // a lane's row of a resident operand, zeros behind the head dimension
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 __device__ inline void load_frag(Vec16<T>* frag, const T* row, int h, int dim, bool valid) {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, DC>;
 #pragma unroll
   for (int ks = 0; ks < L::NS; ks++) {
     const int at = (2 * ks + h) * L::VEC;
@@ -172,10 +174,10 @@ __device__ inline void load_frag(Vec16<T>* frag, const T* row, int h, int dim, b
 }
 
 // lane = row, registers = 32-column blocks: a row's D values as pieces of four
-template <typename T, int DP>
+template <typename T, int DC>
 __device__ inline void store_row(T* row, const f32x16* acc, int h, int dim, float f) {
 #pragma unroll
-  for (int c = 0; c < DP / 32; c++)
+  for (int c = 0; c < DC / 32; c++)
 #pragma unroll
     for (int g = 0; g < 4; g++) {
       const int at = c * 32 + 8 * g + 4 * h;
@@ -200,7 +202,7 @@ __device__ inline void store_row(T* row, const f32x16* acc, int h, int dim, floa
 // The lane's slot of a row is linear in the bits of the row's number, so request i differs from request 0 by an XOR and by whole rows, which go
 // into the instruction's scalar offset: one v_xad a request.
 template <typename T, int DP, int R> struct Fetch {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, DP>;
   static constexpr int NR = R * L::CPR / NT, RPR = 64 / L::CPR;      // requests of a wave, rows of a request
   int wave, lrow;
   int col;
@@ -232,9 +234,9 @@ template <typename T, int DP, int R> struct Fetch {
 // =====================================================================================================================
 // forward.  grid (kv_heads * tiles, key splits); a block owns 128 rows of one sequence and key head, keys stream through LDS.
 // =====================================================================================================================
-template <typename T, int DP, int NB>
+template <typename T, int DP, int DC, int NB>
 __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, DC>;
   constexpr int KT = 32 * NB;
   __shared__ __attribute__((aligned(16))) T sK[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T sV[2][KT * DP];
@@ -254,7 +256,7 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
   const int klast = limit(tile * BR + BR - 1), kend = blockIdx.y + 1 == gridDim.y ? klast : min(klast, kbeg + a.split_keys);
 
   Vec16<T> qf[L::NS];
-  load_frag<T, DP>(qf, (const T*)a.Q + (long)(e.q0 + qi) * a.ldq + (long)(kh * a.group + rc % a.group) * a.hsq, h, dim, r < rows);
+  load_frag<T, DP, DC>(qf, (const T*)a.Q + (long)(e.q0 + qi) * a.ldq + (long)(kh * a.group + rc % a.group) * a.hsq, h, dim, r < rows);
   f32x16 o[L::NC];
 #pragma unroll
   for (int c = 0; c < L::NC; c++)
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
       for (int n = 0; n < NB; n++) {
 #pragma unroll
         for (int i = 0; i < 16; i++) s[n][i] = 0.f;
-        mma_rows<T, DP>(s[n], sK[0], at_r, n * 32, qf);
+        mma_rows<T, DP, DC>(s[n], sK[0], at_r, n * 32, qf);
       }
       if (kb + KT > lim_lo)
 #pragma unroll
@@ -339,11 +341,11 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
             pb[g & 1][j] = (bf16)x;
           }
         };
-        load_cols<T, DP>(v[0], sV[0], at_c, 0);
+        load_cols<T, DP, DC>(v[0], sV[0], at_c, 0);
         probs(0);
 #pragma unroll
         for (int g = 0; g < G; g++) {
-          if (g + 1 < G) load_cols<T, DP>(v[(g + 1) & 1], sV[0], at_c, (g + 1) * 16);
+          if (g + 1 < G) load_cols<T, DP, DC>(v[(g + 1) & 1], sV[0], at_c, (g + 1) * 16);
 #pragma unroll
           for (int c = 0; c < L::NC; c++) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[g & 1][c], pb[g & 1], o[c], 0, 0, 0);
           if (g + 1 < G) probs(g + 1);
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
         for (int n = 0; n < NB; n++) {
 #pragma unroll
           for (int i = 0; i < 16; i++) { s[n][i] = ex2(s[n][i] * c2 - mu); l += s[n][i]; }
-          mma_cols<T, DP>(o, sV[0], at_c, n * 32, s[n]);
+          mma_cols<T, DP, DC>(o, sV[0], at_c, n * 32, s[n]);
         }
       }
     }
@@ -376,11 +378,11 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
   const int hd = rc - qi * a.group;
   if (a.part_o) {
     const long pr = ((long)blockIdx.y * a.kv_heads + kh) * a.rows_q * a.group + (long)e.q0 * a.group + r;
-    store_row<float, DP>(a.part_o + pr * dim, o, h, dim, 1.f);
+    store_row<float, DC>(a.part_o + pr * dim, o, h, dim, 1.f);
     if (h == 0) { a.part_ml[2 * pr] = m; a.part_ml[2 * pr + 1] = l; }
     return;
   }
-  store_row<T, DP>((T*)a.Out + (long)(e.q0 + qi) * a.ldo + (long)(kh * a.group + hd) * a.hso, o, h, dim, l == 0.f ? 0.f : 1.f / l);
+  store_row<T, DC>((T*)a.Out + (long)(e.q0 + qi) * a.ldo + (long)(kh * a.group + hd) * a.hso, o, h, dim, l == 0.f ? 0.f : 1.f / l);
   if (h == 0 && a.lse) a.lse[(long)(kh * a.group + hd) * a.rows_q + e.q0 + qi] = l == 0.f ? INFINITY : m + __log2f(l);
 }
 
@@ -459,9 +461,9 @@ void launch_combine(const PackedArgs& a, int splits, int64_t total, hipStream_t 
 // =====================================================================================================================
 // backward 1: D and dQ, blocked as the forward.
 // =====================================================================================================================
-template <typename T, int DP, int NB>
+template <typename T, int DP, int DC, int NB>
 __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a) {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, DC>;
   constexpr int KT = 32 * NB;
   __shared__ __attribute__((aligned(16))) T sK[2][KT * DP];
   __shared__ __attribute__((aligned(16))) T sV[2][KT * DP];
@@ -482,8 +484,8 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
   const long at = head * a.rows_q + row_g;
 
   Vec16<T> qf[L::NS], gf[L::NS];
-  load_frag<T, DP>(qf, (const T*)a.Q + row_g * a.ldq + head * a.hsq, h, dim, r < rows);
-  load_frag<T, DP>(gf, (const T*)a.dO + row_g * a.lddo + head * a.hsdo, h, dim, r < rows);
+  load_frag<T, DP, DC>(qf, (const T*)a.Q + row_g * a.ldq + head * a.hsq, h, dim, r < rows);
+  load_frag<T, DP, DC>(gf, (const T*)a.dO + row_g * a.lddo + head * a.hsdo, h, dim, r < rows);
   // one key tile: D = sum_j P_ij dP_ij from the tile itself, unrounded (the stored o is off by half a step, which few keys do not average out)
   const bool one_tile = kend <= KT;
   float Dr = 0.f;
@@ -538,8 +540,8 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
         __builtin_amdgcn_s_setprio(1);
-        mma_rows<T, DP>(s, sK[0], at_r, n * 32, qf);
-        mma_rows<T, DP>(dp, sV[0], at_r, n * 32, gf);
+        mma_rows<T, DP, DC>(s, sK[0], at_r, n * 32, qf);
+        mma_rows<T, DP, DC>(dp, sV[0], at_r, n * 32, gf);
         __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = s[i] * c2 - lse;
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = s[i] * (dp[i] - Dr);      // (the scale follows at the end)
         __builtin_amdgcn_s_setprio(1);
-        mma_cols<T, DP>(dq, sK[0], at_c, n * 32, s);
+        mma_cols<T, DP, DC>(dq, sK[0], at_c, n * 32, s);
         __builtin_amdgcn_s_setprio(0);
       }
     }
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
   }
   if (r >= rows) return;
   if (one_tile && h == 0) a.D[at] = Dr;
-  store_row<T, DP>((T*)a.dQ + row_g * a.lddq + head * a.hsdq, dq, h, dim, a.scale);
+  store_row<T, DC>((T*)a.dQ + row_g * a.lddq + head * a.hsdq, dq, h, dim, a.scale);
 }
 
 // =====================================================================================================================
@@ -598,9 +600,9 @@ __device__ inline Parts parts_of(const PackedArgs& a, const Seq& e, int tile, in
   return p;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int DC>
 __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_kernel(const PackedArgs a) {
-  using L = Tile<T, DP>;
+  using L = Tile<T, DP, DC>;
   using F = Fetch<T, DP, RT>;
   constexpr int RING = 4, REQ = 2 * F::NR + 2;      // tiles of the ring, requests of a wave and step
   __shared__ __attribute__((aligned(16))) T sQ[RING][RT * DP];
@@ -621,8 +623,8 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_ke
   const long hd0 = (long)kh * a.group;
 
   Vec16<T> kf[L::NS], vf[L::NS];
-  load_frag<T, DP>(kf, (const T*)a.K + (long)(e.k0 + kc) * a.ldk + (long)kh * a.hsk, h, dim, key < e.lk);
-  load_frag<T, DP>(vf, (const T*)a.V + (long)(e.k0 + kc) * a.ldv + (long)kh * a.hsv, h, dim, key < e.lk);
+  load_frag<T, DP, DC>(kf, (const T*)a.K + (long)(e.k0 + kc) * a.ldk + (long)kh * a.hsk, h, dim, key < e.lk);
+  load_frag<T, DP, DC>(vf, (const T*)a.V + (long)(e.k0 + kc) * a.ldv + (long)kh * a.hsv, h, dim, key < e.lk);
   f32x16 dk[L::NC], dv[L::NC];
 #pragma unroll
   for (int c = 0; c < L::NC; c++)
@@ -688,8 +690,8 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_ke
 #pragma unroll
     for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
     __builtin_amdgcn_s_setprio(1);      // (products first: where the waves of a SIMD meet in the same phase, backward 218 -> 200 us at 676 tokens)
-    mma_rows<T, DP>(s, sQ[0], at_r, 0, kf);
-    mma_rows<T, DP>(dp, sG[0], at_r, 0, vf);
+    mma_rows<T, DP, DC>(s, sQ[0], at_r, 0, kf);
+    mma_rows<T, DP, DC>(dp, sG[0], at_r, 0, vf);
     __builtin_amdgcn_s_setprio(0);
     if (r0 < wall)
 #pragma unroll
@@ -708,19 +710,19 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_ke
       }
     }
     __builtin_amdgcn_s_setprio(1);
-    mma_cols<T, DP>(dv, sG[0], at_c, 0, s);
-    mma_cols<T, DP>(dk, sQ[0], at_c, 0, dp);
+    mma_cols<T, DP, DC>(dv, sG[0], at_c, 0, s);
+    mma_cols<T, DP, DC>(dk, sQ[0], at_c, 0, dp);
     __builtin_amdgcn_s_setprio(0);
   }
   if (key >= e.lk) return;
   if (part.n > 1) {
     float* p = a.part_o + (((long)blockIdx.y * a.kv_heads + kh) * a.rows_k + e.k0 + key) * 2 * dim;
-    store_row<float, DP>(p, dk, h, dim, a.scale);
-    store_row<float, DP>(p + dim, dv, h, dim, 1.f);
+    store_row<float, DC>(p, dk, h, dim, a.scale);
+    store_row<float, DC>(p + dim, dv, h, dim, 1.f);
     return;
   }
-  store_row<T, DP>((T*)a.dK + (long)(e.k0 + key) * a.lddk + (long)kh * a.hsdk, dk, h, dim, a.scale);
-  store_row<T, DP>((T*)a.dV + (long)(e.k0 + key) * a.lddv + (long)kh * a.hsdv, dv, h, dim, 1.f);
+  store_row<T, DC>((T*)a.dK + (long)(e.k0 + key) * a.lddk + (long)kh * a.hsdk, dk, h, dim, a.scale);
+  store_row<T, DC>((T*)a.dV + (long)(e.k0 + key) * a.lddv + (long)kh * a.hsdv, dv, h, dim, 1.f);
 }
 
 // dK, dV of the key tiles in several parts, summed in order.  grid (kv_heads * key tiles, chunks of 16 keys)
@@ -744,6 +746,20 @@ __global__ void __launch_bounds__(NT) packed_parts_kernel(const PackedArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; j++) p[j] = Elem<T>::from_f(v[j]);
   }
+}
+
+// calls f(T{}, columns of a tile row, columns of the products) for a type and head dimension
+template <typename F>
+void for_dim(int dtype, int head_dim, F f) {
+  using std::integral_constant;
+  const auto pick = [&](auto t) {
+    if (head_dim <= 32) f(t, integral_constant<int, 64>{}, integral_constant<int, 32>{});
+    else if (head_dim <= 64) f(t, integral_constant<int, 64>{}, integral_constant<int, 64>{});
+    else if (head_dim <= 96) f(t, integral_constant<int, 128>{}, integral_constant<int, 96>{});
+    else f(t, integral_constant<int, 128>{}, integral_constant<int, 128>{});
+  };
+  if (dtype == CROG_BF16) pick(bf16{});
+  else pick(float{});
 }
 
 bool rows16(const void* p, int64_t ld, int64_t hs, int vec) { return ((uintptr_t)p % 16) == 0 && ld % vec == 0 && hs % vec == 0; }
@@ -773,6 +789,7 @@ extern "C" int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64
   CROG_CHECK_ARG(rows16(Q, ldq, hsq, vec) && rows16(K, ldk, hsk, vec) && rows16(V, ldv, hsv, vec) && rows16(O, ldo, hso, vec) && Q && K && V && O,
                  "packed_attn_fwd: heads of Q / K / V / O must start at 16-byte boundaries");
   CROG_CHECK_ARG(near(ldk, dtype) && near(ldv, dtype), "packed_attn_fwd: 64 key rows must lie within 2 GiB");
+  CROG_CHECK_ARG(splits == 1 || (int64_t)kv_heads * rows_q * group <= 0x7fffffff, "packed_attn_fwd: too many rows for splits");
   CROG_CHECK_ARG(splits >= 1 && splits <= 65535 && (splits == 1 || (partial && split_keys > 0 && split_keys % 64 == 0)),
                  "packed_attn_fwd: %d splits need a workspace and a multiple of 64 keys each (got %d)", splits, split_keys);
   if (n_tiles == 0) return CROG_OK;
@@ -786,13 +803,10 @@ extern "C" int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64
   if (splits > 1) { a.part_o = partial; a.part_ml = partial + (int64_t)splits * total * head_dim; }
   const dim3 grid((unsigned)(n_tiles * kv_heads), splits);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == CROG_BF16) {
-    if (head_dim <= 64) packed_fwd_kernel<bf16, 64, 2><<<grid, NT, 0, s>>>(a);
-    else packed_fwd_kernel<bf16, 128, 2><<<grid, NT, 0, s>>>(a);
-  } else {
-    if (head_dim <= 64) packed_fwd_kernel<float, 64, 1><<<grid, NT, 0, s>>>(a);
-    else packed_fwd_kernel<float, 128, 1><<<grid, NT, 0, s>>>(a);
-  }
+  for_dim(dtype, head_dim, [&](auto t, auto dp, auto dc) {
+    using T = decltype(t);
+    packed_fwd_kernel<T, dp(), dc(), sizeof(T) == 2 ? 2 : 1><<<grid, NT, 0, s>>>(a);
+  });
   CROG_LAUNCH_CHECK();
   if (splits > 1) {
     if (dtype == CROG_BF16) launch_combine<bf16>(a, splits, total, s);
@@ -828,13 +842,10 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
   if (n_row_tiles > 0) {
     a.tiles = row_tiles;
     const unsigned n = (unsigned)(n_row_tiles * kv_heads);
-    if (dtype == CROG_BF16) {
-      if (head_dim <= 64) packed_bwd_dq_kernel<bf16, 64, 2><<<n, NT, 0, s>>>(a);
-      else packed_bwd_dq_kernel<bf16, 128, 2><<<n, NT, 0, s>>>(a);
-    } else {
-      if (head_dim <= 64) packed_bwd_dq_kernel<float, 64, 1><<<n, NT, 0, s>>>(a);
-      else packed_bwd_dq_kernel<float, 128, 1><<<n, NT, 0, s>>>(a);
-    }
+    for_dim(dtype, head_dim, [&](auto t, auto dp, auto dc) {
+      using T = decltype(t);
+      packed_bwd_dq_kernel<T, dp(), dc(), sizeof(T) == 2 ? 2 : 1><<<n, NT, 0, s>>>(a);
+    });
     CROG_LAUNCH_CHECK();
   }
   if (n_key_tiles > 0) {
@@ -843,13 +854,7 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
     a.piece = parts > 1 ? part_steps : 0x7fffff00;
     a.part_o = partial;
     const dim3 n((unsigned)(n_key_tiles * kv_heads), parts);
-    if (dtype == CROG_BF16) {
-      if (head_dim <= 64) packed_bwd_dkdv_kernel<bf16, 64><<<n, NT, 0, s>>>(a);
-      else packed_bwd_dkdv_kernel<bf16, 128><<<n, NT, 0, s>>>(a);
-    } else {
-      if (head_dim <= 64) packed_bwd_dkdv_kernel<float, 64><<<n, NT, 0, s>>>(a);
-      else packed_bwd_dkdv_kernel<float, 128><<<n, NT, 0, s>>>(a);
-    }
+    for_dim(dtype, head_dim, [&](auto t, auto dp, auto dc) { packed_bwd_dkdv_kernel<decltype(t), dp(), dc()><<<n, NT, 0, s>>>(a); });
     CROG_LAUNCH_CHECK();
     if (parts > 1) {
       if (dtype == CROG_BF16) packed_parts_kernel<bf16><<<dim3(n.x, BK / 16), NT, 0, s>>>(a);
