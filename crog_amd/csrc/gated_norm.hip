@@ -385,18 +385,16 @@ extern "C" int crog_gated_norm_fwd(int dtype, const void* x, int64_t ldx, const 
 extern "C" int crog_gated_norm_bwd(int dtype, const void* x, int64_t ldx, const void* y, int64_t ldy, const void* du, int64_t lddu, const void* dh,
                                    int64_t lddh, const float* gate, const float* post_w, const float* post_b, const float* pre_w, int has_post, int has_pre,
                                    int rms, float alpha, int rows, int cols, const float* stats, void* dx, int64_t lddx, void* dy, int64_t lddy, float* slab,
-                                   float* dgate, float* dpost_w, float* dpost_b, float* dpre_w, float* dpre_b, crog_stream_t stream) {
+                                   crog_stream_t stream) {
   CROG_CHECK_ARG(dtype == CROG_F32 || dtype == CROG_BF16, "gated_norm_bwd: dtype must be CROG_F32 or CROG_BF16 (got %d)", dtype);
   CROG_CHECK_ARG(rows >= 0 && cols > 0 && cols <= MAX_COLS, "gated_norm_bwd: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
   if (rows == 0) return CROG_OK;
   CROG_CHECK_ARG(x && y && stats && ldx >= cols && ldy >= cols && (!du || lddu >= cols) && (!dh || lddh >= cols) && (!dx || lddx >= cols) && (!dy || lddy >= cols),
                  "gated_norm_bwd: bad tensors");
   CROG_CHECK_ARG((uintptr_t)stats % 16 == 0, "gated_norm_bwd: stats must be 16-byte aligned");
-  const bool sums = dgate || dpost_w || dpost_b || dpre_w || dpre_b;
-  CROG_CHECK_ARG(!sums || slab, "gated_norm_bwd: the weights' gradients need a slab of crog_gated_norm_slab_floats()");
   GnArgs a{};
   a.x = x; a.y = y; a.du = du; a.dh = dh; a.dx = dx; a.dy = dy; a.gate = gate; a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w;
-  a.stats = const_cast<float*>(stats); a.slab = sums ? slab : nullptr;
+  a.stats = const_cast<float*>(stats); a.slab = slab;
   a.ldx = ldx; a.ldy = ldy; a.lddu = lddu; a.lddh = lddh; a.lddx = lddx; a.lddy = lddy; a.rows = rows; a.cols = cols; a.rms = rms;
   a.has_post = has_post; a.has_pre = has_pre; a.alpha = alpha;
   const int vec = dtype == CROG_BF16 ? 8 : 4;
@@ -404,10 +402,16 @@ extern "C" int crog_gated_norm_bwd(int dtype, const void* x, int64_t ldx, const 
   if (dtype == CROG_BF16) launch_t<bf16>(a, false, vec16, (hipStream_t)stream);
   else launch_t<float>(a, false, vec16, (hipStream_t)stream);
   CROG_LAUNCH_CHECK();
-  if (sums) {
-    gated_norm_sums_kernel<<<cdiv(cols, 16), 16 * RUNS, 0, (hipStream_t)stream>>>(slab, blocks_for(rows, cols), cols, gate, post_w, post_b, has_post, dgate, dpost_w,
-                                                                            dpost_b, dpre_w, dpre_b);
-    CROG_LAUNCH_CHECK();
-  }
+  return CROG_OK;
+}
+
+extern "C" int crog_gated_norm_sums(const float* slab, int rows, int cols, const float* gate, const float* post_w, const float* post_b, int has_post,
+                                    float* dgate, float* dpost_w, float* dpost_b, float* dpre_w, float* dpre_b, crog_stream_t stream) {
+  CROG_CHECK_ARG(rows >= 0 && cols > 0 && cols <= MAX_COLS, "gated_norm_sums: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
+  if (rows == 0 || !(dgate || dpost_w || dpost_b || dpre_w || dpre_b)) return CROG_OK;
+  CROG_CHECK_ARG(slab, "gated_norm_sums: the slab of crog_gated_norm_bwd is missing");
+  gated_norm_sums_kernel<<<cdiv(cols, 16), 16 * RUNS, 0, (hipStream_t)stream>>>(slab, blocks_for(rows, cols), cols, gate, post_w, post_b, has_post, dgate,
+                                                                                dpost_w, dpost_b, dpre_w, dpre_b);
+  CROG_LAUNCH_CHECK();
   return CROG_OK;
 }

@@ -245,15 +245,15 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
   const int tile = a.tiles[2 * ti + 1];
   const Seq e = seq_of(a, a.tiles[2 * ti]);
   const int rows = e.lq * a.group, dim = a.dim;
+  if (tile < 0 || (long)tile * BR >= rows) return;      // (uniform)
   const int r0 = tile * BR + wave * 32, r = r0 + ln;
-  if (tile < 0 || tile * BR >= rows) return;      // (uniform)
   const int off = e.lk - e.lq;
   const int rc = min(r, rows - 1), qi = rc / a.group;
   const int lim = a.causal ? min(max(qi + 1 + off, 0), e.lk) : e.lk;      // the lane's row sees keys [0, lim)
   const auto limit = [&](int row) { return a.causal ? min(max(min(row, rows - 1) / a.group + 1 + off, 0), e.lk) : e.lk; };
   const int lim_lo = limit(r0), lim_hi = r0 < rows ? limit(r0 + 31) : 0;
   const int kbeg = (int)min((long)blockIdx.y * a.split_keys, (long)0x7fffff00);
-  const int klast = limit(tile * BR + BR - 1), kend = blockIdx.y + 1 == gridDim.y ? klast : min(klast, kbeg + a.split_keys);
+  const int klast = limit(tile * BR + BR - 1), kend = blockIdx.y + 1 == gridDim.y ? klast : (int)min((long)klast, (long)kbeg + a.split_keys);
 
   Vec16<T> qf[L::NS];
   load_frag<T, DP, DC>(qf, (const T*)a.Q + (long)(e.q0 + qi) * a.ldq + (long)(kh * a.group + rc % a.group) * a.hsq, h, dim, r < rows);
@@ -472,8 +472,8 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
   const int tile = a.tiles[2 * ti + 1];
   const Seq e = seq_of(a, a.tiles[2 * ti]);
   const int rows = e.lq * a.group, dim = a.dim;
+  if (tile < 0 || (long)tile * BR >= rows) return;
   const int r0 = tile * BR + wave * 32, r = r0 + ln;
-  if (tile < 0 || tile * BR >= rows) return;
   const int off = e.lk - e.lq;
   const int rc = min(r, rows - 1), qi = rc / a.group;
   const int lim = a.causal ? min(max(qi + 1 + off, 0), e.lk) : e.lk;
@@ -594,9 +594,9 @@ __device__ inline Parts parts_of(const PackedArgs& a, const Seq& e, int tile, in
   Parts p;
   const int first = a.causal ? min(max(tile * BK - (e.lk - e.lq), 0), e.lq) : 0;
   const int steps = ((e.lq + RT - 1) / RT - first / RT) * a.group;
-  p.n = min(max((steps + a.piece - 1) / a.piece, 1), a.parts);
+  p.n = min(max((int)(((long)steps + a.piece - 1) / a.piece), 1), a.parts);
   p.begin = (int)min((long)y * a.piece, (long)steps);
-  p.end = y == p.n - 1 ? steps : min(p.begin + a.piece, steps);
+  p.end = y == p.n - 1 ? steps : (int)min((long)p.begin + a.piece, (long)steps);
   return p;
 }
 
@@ -613,8 +613,8 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_ke
   const int tile = a.tiles[2 * ti + 1];
   const Seq e = seq_of(a, a.tiles[2 * ti]);
   const int dim = a.dim;
+  if (tile < 0 || (long)tile * BK >= e.lk) return;      // (uniform)
   const int k0 = tile * BK + wave * 32, key = k0 + ln, kc = min(key, e.lk - 1);
-  if (tile < 0 || tile * BK >= e.lk) return;
   const Parts part = parts_of(a, e, tile, blockIdx.y);
   if ((int)blockIdx.y >= part.n) return;      // (uniform)
   const int off = e.lk - e.lq;
@@ -729,9 +729,10 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_ke
 template <typename T>
 __global__ void __launch_bounds__(NT) packed_parts_kernel(const PackedArgs a) {
   const int kh = blockIdx.x % a.kv_heads, ti = blockIdx.x / a.kv_heads;
-  const int tile = a.tiles[2 * ti + 1], k0 = tile * BK + blockIdx.y * 16;
+  const int tile = a.tiles[2 * ti + 1];
   const Seq e = seq_of(a, a.tiles[2 * ti]);
-  if (tile < 0 || k0 >= e.lk) return;
+  if (tile < 0 || (long)tile * BK + blockIdx.y * 16 >= e.lk) return;
+  const int k0 = tile * BK + blockIdx.y * 16;
   const int n = parts_of(a, e, tile, 0).n;
   if (n == 1) return;
   const int keys = min(16, e.lk - k0), per = 2 * a.dim / 4;

@@ -1302,7 +1302,8 @@ def packed_attention(q, k, v, rows, scale=None):
     """q [rows, heads, dim], k and v [key rows, heads / group, dim], float32 or bfloat16, in the order of `rows` (packed.PackedRows: lengths,
     group, causal); any strides with adjacent columns (others are copied).  -> [rows, heads, dim].  scale: dim ** -0.5 by default.  dim is a
     multiple of 8 up to 128 (float32: of 4).  Rows behind the last sequence give zeros and get zero gradients, whatever they hold.  The same
-    inputs give the same bits (no atomics).  A key or value that is not finite may reach every query of its own sequence, and no other."""
+    inputs give the same bits (no atomics).  A key or value that is not finite may reach every query of its own sequence, and no other; in the
+    backward pass that holds for any row.  Make the plan outside a captured graph."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:
             raise ValueError(f"packed_attention: {name} must be [rows, heads, dim], got {tuple(t.shape)}")
@@ -1400,11 +1401,16 @@ class GatedNormFn(Function):
         dx = _fresh(x) if ctx.needs_input_grad[0] else None
         dy = _fresh(y) if ctx.needs_input_grad[1] else None
         refs = (gate, *(post or (None, None)), *(pre or (None, None)))
-        grads = [_at(r, "G") for r in refs]
-        K.gated_norm_bwd(x, y, du, dh, [_at(r, "P") for r in refs], post is not None, pre is not None, rms, alpha, stats, dx, dy, grads)
-        for r, g in zip(refs, grads):
-            if g is not None:
-                r.done()
+        grads, weights = [_at(r, "G") for r in refs], [_at(r, "P") for r in refs]
+        live = {id(r): r for r, g in zip(refs, grads) if g is not None}
+        slab = K.gated_norm_bwd(x, y, du, dh, weights, post is not None, pre is not None, rms, alpha, stats, dx, dy, bool(live))
+        if live:
+            M, C = stats.shape[0], x.shape[-1]
+            if RT._join_armed:      # this backward pass writes gradients on the weight-gradient stream: behind them, should a weight be shared
+                RT.on_wgrad_stream(lambda: K.gated_norm_sums(slab, M, C, weights, post is not None, grads), slab, tag="ln")
+            else:
+                K.gated_norm_sums(slab, M, C, weights, post is not None, grads)
+            done_joint(live.values())
         return (dx, dy) + none
 
 
@@ -1413,7 +1419,7 @@ def gated_norm(x, y, *, post=None, gate: Optional[WRef] = None, pre=None, res_sc
     h = norm(u) with `pre`; -> (u, h), h None without `pre`.  post / pre: (weight WRef, bias WRef or None); gate: WRef of one factor per column
     (1 without it).  rms: root-mean-square norms (no biases) instead of LayerNorm.  x, y: row matrices [..., C] of one shape and dtype, C up to
     8192; the second norm reads the float32 sum, u and h are rounded once.  The weights' gradients are added into the flat store in a fixed
-    order (same bits every time)."""
+    order (same bits every time).  One weight may stand in several places."""
     K.dcode(x)
     if x.shape != y.shape or x.dtype != y.dtype or x.dim() < 1:
         raise ValueError(f"gated_norm: x and y must have one shape and dtype, got {tuple(x.shape)} {x.dtype} and {tuple(y.shape)} {y.dtype}")

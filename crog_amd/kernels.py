@@ -758,6 +758,13 @@ def same_device(*ts):
             raise RuntimeError(f"a tensor lives on {t.device}, the current device is cuda:{dev}")
 
 
+def plan_used(plan):
+    """Before a launch that reads a plan's tables: on another stream than the one they were made on, their memory must outlive that launch too."""
+    s = stream()
+    if s != plan.made_on and not torch.cuda.is_current_stream_capturing():
+        plan._table.record_stream(torch.cuda.current_stream())
+
+
 def heads16(t: torch.Tensor) -> torch.Tensor:
     """`t` [rows, heads, dim] if every head starts on a 16-byte boundary and its columns are adjacent, else a contiguous copy."""
     s0, s1, s2 = t.stride()
@@ -773,6 +780,7 @@ def packed_attn_fwd(q, k, v, o, lse, rows, scale):
     """q [>= rows.rows_q, kv_heads * group, dim], k, v [>= rows.rows_k, kv_heads, dim]; rows: packed.PackedRows."""
     kv, dim = k.shape[1], k.shape[2]
     splits, piece = rows.splits(kv)
+    plan_used(rows)
     ws = torch.empty(splits * kv * rows.rows_q * rows.group * (dim + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
     check(lib().crog_packed_attn_fwd(dcode(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                                      v.stride(1), o.data_ptr(), o.stride(0), o.stride(1), ptr(lse), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr,
@@ -783,6 +791,7 @@ def packed_attn_fwd(q, k, v, o, lse, rows, scale):
 def packed_attn_bwd(q, k, v, o, do, lse, D, dq, dk, dv, rows, scale):
     kv, dim = k.shape[1], k.shape[2]
     parts, piece = rows.parts(kv)
+    plan_used(rows)
     ws = torch.empty(parts * kv * rows.rows_k * 2 * dim, device=q.device, dtype=torch.float32) if parts > 1 else None
     check(lib().crog_packed_attn_bwd(dcode(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
                                      v.stride(1), o.data_ptr(), o.stride(0), o.stride(1), do.data_ptr(), do.stride(0), do.stride(1), ptr(lse), ptr(D),
@@ -795,9 +804,10 @@ def packed_attn_bwd(q, k, v, o, do, lse, D, dq, dk, dv, rows, scale):
 def rotary(q, k, q_out, k_out, positions, axes, inverse=False):
     """q / k (either may be None): [rows, heads, dim] with adjacent columns; positions [rows, axes]; axes: packed.RotaryAxes."""
     t = q if q is not None else k
+    plan_used(axes)
 
     def three(x):
-        return (None, 0, 0) if x is None else (x.data_ptr(), x.stride(0), x.stride(1))
+        return (None, 0, 0) if x is None else (x.data_ptr(), *x.stride()[:2])
     check(lib().crog_rotary(dcode(t), *three(q), *three(k), *three(q_out), *three(k_out), positions.data_ptr(), positions.stride(0),
                             positions.element_size(), axes.revs_ptr, axes.axis_ptr, t.shape[0], 0 if q is None else q.shape[1],
                             0 if k is None else k.shape[1], t.shape[2], axes.pairs, axes.axes, axes.interleaved, int(inverse), stream()), "rotary")
@@ -810,14 +820,18 @@ def gated_norm_fwd(x, y, weights, has_post, has_pre, rms, alpha, eps, u, h, stat
                                     C, ptr(h), C, ptr(stats), stream()), "gated_norm_fwd")
 
 
-def gated_norm_bwd(x, y, du, dh, weights, has_post, has_pre, rms, alpha, stats, dx, dy, grads):
-    """grads: addresses of the weights' gradients in the order of `weights` (None = not wanted), added onto."""
+def gated_norm_bwd(x, y, du, dh, weights, has_post, has_pre, rms, alpha, stats, dx, dy, sums):
+    """sums: the weights' gradients are wanted; -> the slab that gated_norm_sums takes (None without)."""
     M, C, ldx = mat(x)
-    slab = None
-    if any(g is not None for g in grads):
-        slab = torch.empty(lib().crog_gated_norm_slab_floats(M, C), device=x.device, dtype=torch.float32)
+    slab = torch.empty(lib().crog_gated_norm_slab_floats(M, C), device=x.device, dtype=torch.float32) if sums else None
 
     def two(t):
         return (None, 0) if t is None else (t.data_ptr(), mat(t)[2])
     check(lib().crog_gated_norm_bwd(dcode(x), x.data_ptr(), ldx, y.data_ptr(), mat(y)[2], *two(du), *two(dh), *weights[:4], has_post, has_pre, rms, alpha, M, C,
-                                    ptr(stats), *two(dx), *two(dy), ptr(slab), *grads, stream()), "gated_norm_bwd")
+                                    ptr(stats), *two(dx), *two(dy), ptr(slab), stream()), "gated_norm_bwd")
+    return slab
+
+
+def gated_norm_sums(slab, M, C, weights, has_post, grads):
+    """grads: addresses of the weights' gradients in the order of `weights` (None = not wanted), added onto."""
+    check(lib().crog_gated_norm_sums(slab.data_ptr(), M, C, *weights[:3], has_post, *grads, stream()), "gated_norm_sums")

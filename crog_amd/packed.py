@@ -21,6 +21,11 @@ SPLIT_MIN = 256
 STEP, PART_MIN = 32, 32      # queries of a dK / dV step; steps of a part at least
 
 
+def _stream_of(table: torch.Tensor):
+    """Raw handle of the stream whose allocations the table belongs to."""
+    return torch.cuda.current_stream(table.device).cuda_stream if table.is_cuda else None
+
+
 def _lengths(name: str, lengths: Sequence[int]) -> np.ndarray:
     if isinstance(lengths, torch.Tensor):
         if lengths.is_cuda:
@@ -84,7 +89,7 @@ class PackedRows:
         parts = [np.concatenate([zero, np.cumsum(lq)]), np.concatenate([zero, np.cumsum(lk)]), rt.reshape(-1), kt.reshape(-1)]
         table = torch.from_numpy(np.concatenate(parts).astype(np.int32))
         self._table = table.to(device)      # one copy; the tables lie in it one behind the other
-        self.device = self._table.device
+        self.device, self.made_on = self._table.device, _stream_of(self._table)
         at, addr = 0, []
         for p in parts:
             addr.append(self._table.data_ptr() + 4 * at)
@@ -132,5 +137,5 @@ class RotaryAxes:
         axis = np.repeat(np.arange(len(sizes), dtype=np.int64), sizes).astype(np.int32)
         raw = np.concatenate([revs.view(np.uint8), axis.view(np.uint8)])      # (the doubles first: aligned)
         self._table = torch.from_numpy(raw).to(device)
-        self.device = self._table.device
+        self.device, self.made_on = self._table.device, _stream_of(self._table)
         self.revs_ptr, self.axis_ptr = self._table.data_ptr(), self._table.data_ptr() + 8 * self.pairs

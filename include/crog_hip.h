@@ -622,7 +622,7 @@ int crog_preprocess_u8(const uint8_t* img, const uint8_t* masks, int B, int H, i
  * parts > 1: a key tile's steps - 32 queries of one head each, from the sequence's last back to the first that see it - are walked in up to `parts` pieces of part_steps (the
  * last takes what is left) that meet in a second launch; partial: parts * kv_heads * rows_k * 2 * head_dim floats.
  * Rows outside every sequence are not read and not written.  Non-finite values of a key or value row may reach every query row of its own
- * sequence (also through a probability of zero), never another sequence. */
+ * sequence (also through a probability of zero), never another sequence; in the backward those of any row reach its sequence. */
 int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64_t hsq, const void* K, int64_t ldk, int64_t hsk,
                          const void* V, int64_t ldv, int64_t hsv, void* O, int64_t ldo, int64_t hso, float* lse, const int* cu_q,
                          const int* cu_k, const int* tiles, int n_tiles, int seqs, int rows_q, int rows_k, int kv_heads, int group,
@@ -645,8 +645,9 @@ int crog_rotary(int dtype, const void* Q, int64_t ldq, int64_t hsq, const void* 
 /* The residual between two blocks: z = N(y) * post_w + post_b (has_post; else z = y), u = alpha * x + gate * z, h = N(u) * pre_w + pre_b
  * (has_pre); N = LayerNorm's, or with rms the root-mean-square norm.  Weights fp32 [cols], NULL = 1 (post_w, pre_w, gate) or 0 (post_b,
  * pre_b); cols <= 8192.  The second norm reads the fp32 sum.  stats: NULL or [rows][4] floats for the backward.
- * Backward: du, dh may be NULL (no gradient); dx, dy may be NULL (not wanted); the weights' gradients are ADDED onto what their buffers hold
- * (NULL = not wanted), through slab, crog_gated_norm_slab_floats(rows, cols) floats of scratch, in a fixed order. */
+ * Backward: du, dh may be NULL (no gradient); dx, dy and slab may be NULL (not wanted).  slab: crog_gated_norm_slab_floats(rows, cols) floats of
+ * column sums, from which crog_gated_norm_sums forms the weights' gradients in a fixed order and ADDS them onto what their buffers hold (NULL =
+ * not wanted; two of them may be the same buffer). */
 int crog_gated_norm_slab_floats(int rows, int cols);
 int crog_gated_norm_fwd(int dtype, const void* x, int64_t ldx, const void* y, int64_t ldy, const float* gate, const float* post_w,
                         const float* post_b, const float* pre_w, const float* pre_b, int has_post, int has_pre, int rms, float alpha,
@@ -654,8 +655,9 @@ int crog_gated_norm_fwd(int dtype, const void* x, int64_t ldx, const void* y, in
 int crog_gated_norm_bwd(int dtype, const void* x, int64_t ldx, const void* y, int64_t ldy, const void* du, int64_t lddu,
                         const void* dh, int64_t lddh, const float* gate, const float* post_w, const float* post_b, const float* pre_w,
                         int has_post, int has_pre, int rms, float alpha, int rows, int cols, const float* stats, void* dx, int64_t lddx,
-                        void* dy, int64_t lddy, float* slab, float* dgate, float* dpost_w, float* dpost_b, float* dpre_w,
-                        float* dpre_b, crog_stream_t stream);
+                        void* dy, int64_t lddy, float* slab, crog_stream_t stream);
+int crog_gated_norm_sums(const float* slab, int rows, int cols, const float* gate, const float* post_w, const float* post_b, int has_post,
+                         float* dgate, float* dpost_w, float* dpost_b, float* dpre_w, float* dpre_b, crog_stream_t stream);
 
 #ifdef __cplusplus
 }

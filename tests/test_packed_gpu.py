@@ -128,17 +128,36 @@ def test_attention_matches_the_formula(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
-def test_attention_scale_and_sharp_scores(dtype):
-    """Scores of hundreds: one key takes everything, and the running maximum jumps by more than its slack again and again."""
+@pytest.mark.parametrize("scale", [0.7, -0.25, 0.0])
+def test_attention_scale_and_sharp_scores(scale, dtype):
+    """Scores of hundreds: one key takes everything, and the running maximum jumps by more than its slack again and again; a negative scale; a
+    scale of zero, whose probabilities are all the same."""
     from crog_amd.packed import PackedRows
     lq = [300]
     rows = PackedRows(lq, causal=True)
     q, k, v, do = (dev(300, 1, 64, dtype=dtype, seed=i, scale=s) for i, s in ((1, 3.0), (2, 3.0), (3, 1.0), (4, 1.0)))
     k = (k.float() * torch.linspace(0.1, 3, 300, device="cuda")[:, None, None]).to(dtype)
-    got = run_attention(q, k, v, do, rows, 0.7)
-    want, bound = attention_reference(q, k, v, do, lq, lq, True, 0.7)
+    got = run_attention(q, k, v, do, rows, scale)
+    want, bound = attention_reference(q, k, v, do, lq, lq, True, scale)
     for n in got:
         within(got[n], want[n], bound[n], n)
+
+
+def test_attention_rows_far_apart():
+    """Rows 4 MiB apart: offsets beyond 32 bits; and rows further apart than a tile's 32-bit offsets, which are copied first."""
+    from crog_amd.packed import PackedRows
+    rows = PackedRows([3, 2], [1100, 7], causal=True)
+    q, do = dev(5, 2, 64, dtype=torch.bfloat16, seed=1), dev(5, 2, 64, dtype=torch.bfloat16, seed=2)
+    k, v = dev(1107, 2, 64, dtype=torch.bfloat16, seed=3), dev(1107, 2, 64, dtype=torch.bfloat16, seed=4)
+    want = run_attention(q, k, v, do, rows)
+    wide = torch.empty(1107, 1 << 21, device="cuda", dtype=torch.bfloat16)
+    far_k, far_v = wide[:, :128].view(1107, 2, 64).copy_(k), wide[:, 128:256].view(1107, 2, 64).copy_(v)
+    got = run_attention(q, far_k, far_v, do, rows)
+    assert all(torch.equal(got[n], want[n]) for n in got)
+    lone = torch.empty(3, 1 << 23, device="cuda", dtype=torch.bfloat16)[:, :128].view(3, 2, 64)
+    few = PackedRows([3])
+    lone.copy_(k[:3])
+    assert torch.equal(run_attention(q[:3], lone, lone, do[:3], few)["o"], run_attention(q[:3], k[:3], k[:3], do[:3], few)["o"])
 
 
 def test_attention_strides_and_alignment():
@@ -261,7 +280,10 @@ def test_attention_on_another_stream():
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         got = run_attention(q, k, v, do, rows)
+    rows = None      # (the plan was made on the other stream: its tables' memory goes to no new tensor before the launches have read them)
+    filler = [torch.full((64,), 0x7fffffff, device="cuda", dtype=torch.int32) for _ in range(64)]
     side.synchronize()
+    del filler
     assert all(torch.equal(got[n], want[n]) for n in got)
 
 
@@ -454,6 +476,18 @@ def test_gated_norm_accumulates_views_and_missing_gradients():
     assert all(torch.equal(s, t) for s, t in zip(only_u, zero_h))
     only_h, zero_u = grads(x, y, None, dh), grads(x, y, torch.zeros_like(du), dh)
     assert all(torch.equal(s, t) for s, t in zip(only_h, zero_u))
+    # one weight in several places: its gradient is the sum over the places
+    st.zero_grad()
+    xx, yy = (t.detach().requires_grad_() for t in (x, y))
+    u, h = Fn.gated_norm(xx, yy, post=(r["post_w"], r["post_b"]), gate=r["post_w"], pre=(r["post_w"], r["post_b"]), res_scale=0.5)
+    torch.autograd.grad((u, h), (xx, yy), (du, dh))
+    shared = {n: r[n].grad().clone() for n in ("post_w", "post_b")}
+    want, bound = norm_reference(x.flatten(0, 1), y.flatten(0, 1), du.flatten(0, 1), dh.flatten(0, 1),
+                                 {"gate": m.post_w.detach(), "post_w": m.post_w.detach(), "pre_w": m.post_w.detach(), "post_b": m.post_b.detach(), "pre_b": m.post_b.detach()},
+                                 True, True, False, 0.5, 1e-5)
+    for n, parts in (("post_w", ("gate", "post_w", "pre_w")), ("post_b", ("post_b", "pre_b"))):
+        total = sum(want[p] for p in parts)
+        within(shared[n], total, sum(bound[p] for p in parts) + 4 * U * sum(want[p].abs() for p in parts), n)
     # two passes without clearing add up (to one rounding each); a frozen weight is left alone
     st.zero_grad()
     m.post_w.requires_grad_(False)

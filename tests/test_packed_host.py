@@ -167,7 +167,10 @@ def test_c_entries_refuse_before_any_launch():
     g = [1, p, 64, p, 64, None, None, None, None, None, 0, 1, 0, 1.0, 1e-5, 4, 64, p, 64, p, 64, None, None]
     for at, v in ((0, 2), (1, None), (2, 63), (15, -1), (16, 0), (16, 8193), (17, None), (19, None), (21, p + 4)):
         assert lib.crog_gated_norm_fwd(*g[:at], v, *g[at + 1:]) == -1, at
-    b = [1, p, 64, p, 64, p, 64, p, 64, None, None, None, None, 0, 1, 0, 1.0, 4, 64, p, p, 64, p, 64, None, None, None, None, None, None, None]
-    for at, v in ((0, 2), (1, None), (17, -1), (18, 8193), (19, None), (19, p + 4), (25, p), (21, 63)):
+    b = [1, p, 64, p, 64, p, 64, p, 64, None, None, None, None, 0, 1, 0, 1.0, 4, 64, p, p, 64, p, 64, None, None]
+    for at, v in ((0, 2), (1, None), (17, -1), (18, 8193), (19, None), (19, p + 4), (21, 63)):
         assert lib.crog_gated_norm_bwd(*b[:at], v, *b[at + 1:]) == -1, at
+    c = [p, 4, 64, None, None, None, 0, p, None, None, None, None, None]
+    for at, v in ((0, None), (1, -1), (2, 0), (2, 8193)):
+        assert lib.crog_gated_norm_sums(*c[:at], v, *c[at + 1:]) == -1, at
     assert lib.crog_gated_norm_slab_floats(0, 64) == 0 and lib.crog_gated_norm_slab_floats(10 ** 6, 64) == 512 * 4 * 64
