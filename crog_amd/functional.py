@@ -1304,6 +1304,17 @@ def packed_attention(q, k, v, rows, scale=None):
     multiple of 8 up to 128 (float32: of 4).  Rows behind the last sequence give zeros and get zero gradients, whatever they hold.  The same
     inputs give the same bits (no atomics).  A key or value that is not finite may reach every query of its own sequence, and no other; in the
     backward pass that holds for any row.  Make the plan outside a captured graph."""
+    qs, ks, dt, group = q.shape, k.shape, q.dtype, rows.group
+    # (one condition for the calls that are right; what is wrong with another is found out behind it)
+    if not (len(qs) == 3 == len(ks) and ks == v.shape and k.dtype == dt == v.dtype and qs[2] == ks[2] and qs[1] == ks[1] * group and ks[1] > 0
+            and 0 < qs[2] <= 128 and qs[2] % (16 // q.element_size()) == 0 and qs[0] >= rows.rows_q and ks[0] >= rows.rows_k
+            and (dt is torch.bfloat16 or dt is torch.float32) and (scale is None or math.isfinite(scale))):
+        _refuse_attention(q, k, v, rows, scale)
+    K.same_device(q, k, v, rows._table)
+    return PackedAttentionFn.apply(q, k, v, rows, qs[2] ** -0.5 if scale is None else float(scale))
+
+
+def _refuse_attention(q, k, v, rows, scale):
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:
             raise ValueError(f"packed_attention: {name} must be [rows, heads, dim], got {tuple(t.shape)}")
@@ -1317,10 +1328,7 @@ def packed_attention(q, k, v, rows, scale=None):
         raise ValueError(f"packed_attention: the head dimension must be a multiple of {vec} up to 128 for {q.dtype}, got {dim}")
     if q.shape[0] < rows.rows_q or k.shape[0] < rows.rows_k:
         raise ValueError(f"packed_attention: the plan has {rows.rows_q} query and {rows.rows_k} key rows, the tensors {q.shape[0]} and {k.shape[0]}")
-    if scale is not None and not math.isfinite(scale):
-        raise ValueError("packed_attention: scale must be finite")
-    K.same_device(q, k, v, rows._table)
-    return PackedAttentionFn.apply(q, k, v, rows, float(dim ** -0.5 if scale is None else scale))
+    raise ValueError(f"packed_attention: scale must be finite, got {scale}")
 
 
 class RotaryFn(Function):
@@ -1333,10 +1341,15 @@ class RotaryFn(Function):
 
     @staticmethod
     def _turn(q, k, positions, axes, inverse):
-        q, k = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (q, k))
-        qo, ko = (None if t is None else _fresh(t) for t in (q, k))
+        qo = ko = None
+        if q is not None:
+            q = q if q.stride(2) == 1 else q.contiguous()
+            qo = _fresh(q)
+        if k is not None:
+            k = k if k.stride(2) == 1 else k.contiguous()
+            ko = _fresh(k)
         if q is not None or k is not None:
-            K.rotary(q, k, qo, ko, positions, axes, inverse=inverse)
+            K.rotary(q, k, qo, ko, positions, axes, inverse)
         return qo, ko
 
     @staticmethod

@@ -776,27 +776,30 @@ def heads16(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _heads(t: torch.Tensor):
+    """(address, row stride, head stride) of a [rows, heads, dim] tensor"""
+    s = t.stride()
+    return t.data_ptr(), s[0], s[1]
+
+
 def packed_attn_fwd(q, k, v, o, lse, rows, scale):
     """q [>= rows.rows_q, kv_heads * group, dim], k, v [>= rows.rows_k, kv_heads, dim]; rows: packed.PackedRows."""
-    kv, dim = k.shape[1], k.shape[2]
+    _, kv, dim = k.shape
     splits, piece = rows.splits(kv)
     plan_used(rows)
     ws = torch.empty(splits * kv * rows.rows_q * rows.group * (dim + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
-    check(lib().crog_packed_attn_fwd(dcode(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                     v.stride(1), o.data_ptr(), o.stride(0), o.stride(1), ptr(lse), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr,
+    check(lib().crog_packed_attn_fwd(dcode(q), *_heads(q), *_heads(k), *_heads(v), *_heads(o), ptr(lse), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr,
                                      rows.n_row_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, splits, piece,
                                      ptr(ws), stream()), "packed_attn_fwd")
 
 
 def packed_attn_bwd(q, k, v, o, do, lse, D, dq, dk, dv, rows, scale):
-    kv, dim = k.shape[1], k.shape[2]
+    _, kv, dim = k.shape
     parts, piece = rows.parts(kv)
     plan_used(rows)
     ws = torch.empty(parts * kv * rows.rows_k * 2 * dim, device=q.device, dtype=torch.float32) if parts > 1 else None
-    check(lib().crog_packed_attn_bwd(dcode(q), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                     v.stride(1), o.data_ptr(), o.stride(0), o.stride(1), do.data_ptr(), do.stride(0), do.stride(1), ptr(lse), ptr(D),
-                                     dq.data_ptr(), dq.stride(0), dq.stride(1), dk.data_ptr(), dk.stride(0), dk.stride(1), dv.data_ptr(), dv.stride(0),
-                                     dv.stride(1), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr, rows.n_row_tiles, rows.key_tiles_ptr,
+    check(lib().crog_packed_attn_bwd(dcode(q), *_heads(q), *_heads(k), *_heads(v), *_heads(o), *_heads(do), ptr(lse), ptr(D), *_heads(dq), *_heads(dk),
+                                     *_heads(dv), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr, rows.n_row_tiles, rows.key_tiles_ptr,
                                      rows.n_key_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, parts, piece, ptr(ws),
                                      stream()), "packed_attn_bwd")
 
@@ -806,11 +809,11 @@ def rotary(q, k, q_out, k_out, positions, axes, inverse=False):
     t = q if q is not None else k
     plan_used(axes)
 
-    def three(x):
-        return (None, 0, 0) if x is None else (x.data_ptr(), *x.stride()[:2])
-    check(lib().crog_rotary(dcode(t), *three(q), *three(k), *three(q_out), *three(k_out), positions.data_ptr(), positions.stride(0),
+    none = (None, 0, 0)
+    check(lib().crog_rotary(dcode(t), *(none if q is None else _heads(q)), *(none if k is None else _heads(k)), *(none if q is None else _heads(q_out)),
+                            *(none if k is None else _heads(k_out)), positions.data_ptr(), positions.stride(0),
                             positions.element_size(), axes.revs_ptr, axes.axis_ptr, t.shape[0], 0 if q is None else q.shape[1],
-                            0 if k is None else k.shape[1], t.shape[2], axes.pairs, axes.axes, axes.interleaved, int(inverse), stream()), "rotary")
+                            0 if k is None else k.shape[1], t.shape[2], axes.pairs, axes.axes, axes.interleaved, inverse, stream()), "rotary")
 
 
 def gated_norm_fwd(x, y, weights, has_post, has_pre, rms, alpha, eps, u, h, stats):
