@@ -24,6 +24,14 @@ struct RotArgs {
   int rows, heads_q, heads_k, dim, pairs, axes, pos64, inverse;
 };
 
+// The fused steps are written out: left to the compiler, the variants below fused different ones of the two products, and the same pair came out
+// one fp32 step apart (now and then a bf16 one) with another alignment.
+__device__ inline void turn(float& x, float& y, float c, float s) {
+  const float x1 = fmaf(-y, s, x * c);
+  y = fmaf(x, s, y * c);
+  x = x1;
+}
+
 // PV: pairs of one work item (16 bytes of each half, or PV interleaved pairs)
 template <typename T, int PV, bool INTER, int TOK>
 __global__ void __launch_bounds__(NT) rotary_kernel(const RotArgs a) {
@@ -68,9 +76,11 @@ __global__ void __launch_bounds__(NT) rotary_kernel(const RotArgs a) {
       __builtin_memcpy(v, __builtin_assume_aligned(src + 2 * p0, PV == 1 ? sizeof(T) : 16), sizeof(v));
 #pragma unroll
       for (int e = 0; e < PV; e++) {
-        const float c = sc[t][p0 + e][0], s = sc[t][p0 + e][1], x = Elem<T>::to_f(v[2 * e]), y = Elem<T>::to_f(v[2 * e + 1]);
-        v[2 * e] = Elem<T>::from_f(x * c - y * s);
-        v[2 * e + 1] = Elem<T>::from_f(y * c + x * s);
+        const float c = sc[t][p0 + e][0], s = sc[t][p0 + e][1];
+        float x = Elem<T>::to_f(v[2 * e]), y = Elem<T>::to_f(v[2 * e + 1]);
+        turn(x, y, c, s);
+        v[2 * e] = Elem<T>::from_f(x);
+        v[2 * e + 1] = Elem<T>::from_f(y);
       }
       __builtin_memcpy(__builtin_assume_aligned(dst + 2 * p0, PV == 1 ? sizeof(T) : 16), v, sizeof(v));
     } else {
@@ -80,9 +90,11 @@ __global__ void __launch_bounds__(NT) rotary_kernel(const RotArgs a) {
       __builtin_memcpy(y, __builtin_assume_aligned(src + a.pairs + p0, AL), sizeof(y));
 #pragma unroll
       for (int e = 0; e < PV; e++) {
-        const float c = sc[t][p0 + e][0], s = sc[t][p0 + e][1], xf = Elem<T>::to_f(x[e]), yf = Elem<T>::to_f(y[e]);
-        x[e] = Elem<T>::from_f(xf * c - yf * s);
-        y[e] = Elem<T>::from_f(yf * c + xf * s);
+        const float c = sc[t][p0 + e][0], s = sc[t][p0 + e][1];
+        float xf = Elem<T>::to_f(x[e]), yf = Elem<T>::to_f(y[e]);
+        turn(xf, yf, c, s);
+        x[e] = Elem<T>::from_f(xf);
+        y[e] = Elem<T>::from_f(yf);
       }
       __builtin_memcpy(__builtin_assume_aligned(dst + p0, AL), x, sizeof(x));
       __builtin_memcpy(__builtin_assume_aligned(dst + a.pairs + p0, AL), y, sizeof(y));
