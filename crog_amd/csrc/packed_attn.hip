@@ -459,7 +459,7 @@ void launch_combine(const PackedArgs& a, int splits, int64_t total, hipStream_t 
 }
 
 // =====================================================================================================================
-// backward 1: D and dQ, blocked as the forward.
+// backward 1: D and dQ, blocked as the forward, its few rows over long keys cut in the same way (the float sums meet in packed_dq_sum_kernel).
 // =====================================================================================================================
 template <typename T, int DP, int DC, int NB>
 __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a) {
@@ -479,17 +479,18 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
   const int lim = a.causal ? min(max(qi + 1 + off, 0), e.lk) : e.lk;
   const auto limit = [&](int row) { return a.causal ? min(max(min(row, rows - 1) / a.group + 1 + off, 0), e.lk) : e.lk; };
   const int lim_lo = limit(r0), lim_hi = r0 < rows ? limit(r0 + 31) : 0;
-  const int kend = limit(tile * BR + BR - 1);
+  const int klast = limit(tile * BR + BR - 1), kbeg = (int)min((long)blockIdx.y * a.split_keys, (long)0x7fffff00);
+  const int kend = blockIdx.y + 1 == gridDim.y ? klast : (int)min((long)klast, (long)kbeg + a.split_keys);
   const long row_g = e.q0 + qi, head = (long)kh * a.group + rc % a.group;
   const long at = head * a.rows_q + row_g;
 
   Vec16<T> qf[L::NS], gf[L::NS];
   load_frag<T, DP, DC>(qf, (const T*)a.Q + row_g * a.ldq + head * a.hsq, h, dim, r < rows);
   load_frag<T, DP, DC>(gf, (const T*)a.dO + row_g * a.lddo + head * a.hsdo, h, dim, r < rows);
-  // one key tile: D = sum_j P_ij dP_ij from the tile itself, unrounded (the stored o is off by half a step, which few keys do not average out)
-  const bool one_tile = kend <= KT;
+  // D = dO . o; of a row that sees the first key tile alone, sum_j P_ij dP_ij from the tile itself, unrounded (the stored o is off by half a step,
+  // which few keys do not average out: sequences of up to 147 causal rows had dQ off by 0.0026 of its norm, 0.0024 with this)
   float Dr = 0.f;
-  if (!one_tile) {
+  if (lim_hi > KT) {
     const T* op = (const T*)a.O + row_g * a.ldo + head * a.hso;
 #pragma unroll
     for (int ks = 0; ks < L::NS; ks++) {
@@ -501,7 +502,6 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
       }
     }
     Dr = xor32_sum(Dr);
-    if (h == 0 && r < rows) a.D[at] = Dr;
   }
   const float lse = a.lse[at], c2 = a.scale * LOG2E;
   const int rows_at = L::rows_at(lane), cols_at = L::cols_at(lane);
@@ -516,14 +516,16 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
   Fetch<T, DP, KT> fk, fv;
   fk.init(wave, lane, a.ldk);
   fv.init(wave, lane, a.ldv);
-  if (kend > 0) {
-    fk.get(lds_k, kg, e.lk, dim);
-    fv.get(lds_v, vg, e.lk, dim);
+  kg += (long)kbeg * a.ldk;
+  vg += (long)kbeg * a.ldv;
+  if (kbeg < kend) {
+    fk.get(lds_k, kg, e.lk - kbeg, dim);
+    fv.get(lds_v, vg, e.lk - kbeg, dim);
   }
   wait_vmcnt<0>();
   __syncthreads();
   int buf = 0;
-  for (int kb = 0; kb < kend; kb += KT, buf ^= 1) {
+  for (int kb = kbeg; kb < kend; kb += KT, buf ^= 1) {
     const bool more = kb + KT < kend;
     if (more) {      // (the barrier below: every wave is done with the other buffer)
       kg += KT * a.ldk;
@@ -552,13 +554,15 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
         for (int i = 0; i < 16; i++) s[i] = ex2(s[i]);
       };
       f32x16 s, dp;
-      if (one_tile) {
+      if (kb == 0 && lim_lo <= KT) {
+        float d = 0.f;
         for (int n = 0; n < NB; n++) {
           probs(n, s, dp);
 #pragma unroll
-          for (int i = 0; i < 16; i++) Dr += s[i] * dp[i];
+          for (int i = 0; i < 16; i++) d += s[i] * dp[i];
         }
-        Dr = xor32_sum(Dr);
+        d = xor32_sum(d);
+        Dr = lim <= KT ? d : Dr;
       }
 #pragma unroll
       for (int n = 0; n < NB; n++) {
@@ -574,8 +578,29 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
     __syncthreads();
   }
   if (r >= rows) return;
-  if (one_tile && h == 0) a.D[at] = Dr;
+  if (h == 0 && blockIdx.y == 0) a.D[at] = Dr;
+  if (a.part_o) {
+    store_row<float, DC>(a.part_o + ((long)blockIdx.y * a.kv_heads * a.group * a.rows_q + at) * dim, dq, h, dim, a.scale);
+    return;
+  }
   store_row<T, DC>((T*)a.dQ + row_g * a.lddq + head * a.hsdq, dq, h, dim, a.scale);
+}
+
+// dQ = the splits' sums in order.  16 threads a row of four columns each, twice
+template <typename T>
+__global__ void __launch_bounds__(NT) packed_dq_sum_kernel(const PackedArgs a, int splits) {
+  const long total = (long)a.kv_heads * a.group * a.rows_q, at = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const long head = at / a.rows_q, row = at - head * a.rows_q;
+  // rows behind the last sequence have no partial result and stay as they are
+  if (at >= total || row >= min(a.cu_q[a.seqs], a.rows_q)) return;
+  for (int c = (threadIdx.x & 15) * 4; c < a.dim; c += 64) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int z = 0; z < splits; z++) v += *reinterpret_cast<const f32x4*>(a.part_o + (z * total + at) * a.dim + c);
+    T* p = (T*)a.dQ + row * a.lddq + head * a.hsdq + c;
+#pragma unroll
+    for (int j = 0; j < 4; j++) p[j] = Elem<T>::from_f(v[j]);
+  }
 }
 
 // =====================================================================================================================
@@ -822,13 +847,15 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
                                     const float* lse, float* D, void* dQ, int64_t lddq, int64_t hsdq, void* dK, int64_t lddk, int64_t hsdk, void* dV,
                                     int64_t lddv, int64_t hsdv, const int* cu_q, const int* cu_k, const int* row_tiles, int n_row_tiles,
                                     const int* key_tiles, int n_key_tiles, int seqs, int rows_q, int rows_k, int kv_heads, int group, int head_dim,
-                                    float scale, int causal, int parts, int part_steps, float* partial, crog_stream_t stream) {
+                                    float scale, int causal, int splits, int split_keys, int parts, int part_steps, float* partial, crog_stream_t stream) {
   if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_row_tiles, cu_q, cu_k, row_tiles)) return rc;
   if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_key_tiles, cu_q, cu_k, key_tiles)) return rc;
   const int vec = dtype == CROG_BF16 ? 8 : 4;
   CROG_CHECK_ARG(rows16(Q, ldq, hsq, vec) && rows16(K, ldk, hsk, vec) && rows16(V, ldv, hsv, vec) && rows16(O, ldo, hso, vec) && rows16(dO, lddo, hsdo, vec) &&
                  rows16(dQ, lddq, hsdq, vec) && rows16(dK, lddk, hsdk, vec) && rows16(dV, lddv, hsdv, vec) && Q && K && V && O && dO && lse && D && dQ && dK && dV,
                  "packed_attn_bwd: heads of Q / K / V / O / dO and the gradients must start at 16-byte boundaries");
+  CROG_CHECK_ARG(splits >= 1 && splits <= 65535 && (splits == 1 || (partial && split_keys > 0 && split_keys % 64 == 0)),
+                 "packed_attn_bwd: %d splits need a workspace and a multiple of 64 keys each (got %d)", splits, split_keys);
   CROG_CHECK_ARG(parts >= 1 && parts <= 65535 && (parts == 1 || (part_steps > 0 && partial)),
                  "packed_attn_bwd: %d parts need a workspace and a number of steps each (got %d)", parts, part_steps);
   CROG_CHECK_ARG(near(ldk, dtype) && near(ldv, dtype) && near(ldq, dtype) && near(lddo, dtype),
@@ -842,12 +869,20 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
   hipStream_t s = (hipStream_t)stream;
   if (n_row_tiles > 0) {
     a.tiles = row_tiles;
-    const unsigned n = (unsigned)(n_row_tiles * kv_heads);
+    a.split_keys = splits > 1 ? split_keys : 0x7fffff00;
+    a.part_o = splits > 1 ? partial : nullptr;
+    const dim3 n((unsigned)(n_row_tiles * kv_heads), splits);
     for_dim(dtype, head_dim, [&](auto t, auto dp, auto dc) {
       using T = decltype(t);
       packed_bwd_dq_kernel<T, dp(), dc(), sizeof(T) == 2 ? 2 : 1><<<n, NT, 0, s>>>(a);
     });
     CROG_LAUNCH_CHECK();
+    if (splits > 1) {
+      const unsigned blocks = (unsigned)cdiv((int64_t)kv_heads * group * rows_q, 16);
+      if (dtype == CROG_BF16) packed_dq_sum_kernel<bf16><<<blocks, NT, 0, s>>>(a, splits);
+      else packed_dq_sum_kernel<float><<<blocks, NT, 0, s>>>(a, splits);
+      CROG_LAUNCH_CHECK();
+    }
   }
   if (n_key_tiles > 0) {
     a.tiles = key_tiles;

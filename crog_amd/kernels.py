@@ -785,7 +785,7 @@ def _heads(t: torch.Tensor):
 def packed_attn_fwd(q, k, v, o, lse, rows, scale):
     """q [>= rows.rows_q, kv_heads * group, dim], k, v [>= rows.rows_k, kv_heads, dim]; rows: packed.PackedRows."""
     _, kv, dim = k.shape
-    splits, piece = rows.splits(kv)
+    splits, piece = rows.splits(kv, q.element_size())
     plan_used(rows)
     ws = torch.empty(splits * kv * rows.rows_q * rows.group * (dim + 2), device=q.device, dtype=torch.float32) if splits > 1 else None
     check(lib().crog_packed_attn_fwd(dcode(q), *_heads(q), *_heads(k), *_heads(v), *_heads(o), ptr(lse), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr,
@@ -795,13 +795,15 @@ def packed_attn_fwd(q, k, v, o, lse, rows, scale):
 
 def packed_attn_bwd(q, k, v, o, do, lse, D, dq, dk, dv, rows, scale):
     _, kv, dim = k.shape
-    parts, piece = rows.parts(kv)
+    size = q.element_size()
+    (splits, keys), (parts, steps) = rows.splits(kv, size), rows.parts(kv, size)
     plan_used(rows)
-    ws = torch.empty(parts * kv * rows.rows_k * 2 * dim, device=q.device, dtype=torch.float32) if parts > 1 else None
+    floats = max(splits * kv * rows.group * rows.rows_q * dim if splits > 1 else 0, parts * kv * rows.rows_k * 2 * dim if parts > 1 else 0)
+    ws = torch.empty(floats, device=q.device, dtype=torch.float32) if floats else None
     check(lib().crog_packed_attn_bwd(dcode(q), *_heads(q), *_heads(k), *_heads(v), *_heads(o), *_heads(do), ptr(lse), ptr(D), *_heads(dq), *_heads(dk),
                                      *_heads(dv), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr, rows.n_row_tiles, rows.key_tiles_ptr,
-                                     rows.n_key_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, parts, piece, ptr(ws),
-                                     stream()), "packed_attn_bwd")
+                                     rows.n_key_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, splits, keys, parts, steps,
+                                     ptr(ws), stream()), "packed_attn_bwd")
 
 
 def rotary(q, k, q_out, k_out, positions, axes, inverse=False):

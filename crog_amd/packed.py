@@ -14,11 +14,14 @@ import torch
 
 TILE = 128      # rows (query rows x heads of a group) of a forward / dQ block of csrc/packed_attn.hip
 KEY_TILE = 128  # keys of a dK / dV block
-# Key splits of the forward pass: with fewer blocks than this, a long key axis is cut into pieces so that every CU has work (256 CUs, two blocks
-# each); a piece is at least SPLIT_MIN keys.
+# Long chains of work are cut where there are too few blocks to fill the device (256 CUs, two blocks each): the keys that a block of the forward or
+# dQ pass walks over, the queries that a block of the dK / dV pass walks over.  The pieces meet in a second launch, which costs 4 to 8 us, so a piece
+# has at least SPLIT_MIN keys or PART_MIN steps (by the bytes of an element; fp32 products take eight times as long).  100 keys over 4000 queries of 8
+# heads, bf16: dK / dV 27 us in one part, 17 + 4 in two; one token over 8192 keys, 8 key heads: 85 us in one piece, 11 + 6 in 32.  Twice, four times
+# and eight times as many blocks were no faster or slower.
 FILL_BLOCKS = 512
-SPLIT_MIN = 256
-STEP, PART_MIN = 32, 32      # queries of a dK / dV step; steps of a part at least
+SPLIT_MIN = {2: 256, 4: 128}
+STEP, PART_MIN = 32, {2: 8, 4: 4}      # queries of a dK / dV step
 
 
 def _stream_of(table: torch.Tensor):
@@ -96,23 +99,22 @@ class PackedRows:
             at += len(p)
         self.cu_q_ptr, self.cu_k_ptr, self.row_tiles_ptr, self.key_tiles_ptr = addr
 
-    def splits(self, kv_heads: int):
-        """(pieces, keys of a piece) of the forward pass's key axis.  A single query over 8192 keys of 8 heads would be 8 blocks on 256 CUs;
-        in pieces of 256 keys it is 256.  Enough blocks, or short keys: one piece, no second launch."""
+    def splits(self, kv_heads: int, size: int):
+        """(pieces, keys of a piece) of the forward and dQ passes' key axis; size: bytes of an element.  A single query over 8192 keys of 8 heads
+        would be 8 blocks on 256 CUs; in pieces of 256 keys it is 256.  Enough blocks, or short keys: one piece, no second launch."""
         blocks = max(self.n_row_tiles * kv_heads, 1)
-        n = min(-(-FILL_BLOCKS // blocks), -(-self.max_k // SPLIT_MIN))
+        n = min(-(-FILL_BLOCKS // blocks), self.max_k // SPLIT_MIN[size])
         if n <= 1:
             return 1, 0
         piece = -(-self.max_k // n)
         piece = -(-piece // 64) * 64
         return -(-self.max_k // piece), piece
 
-
-    def parts(self, kv_heads: int):
+    def parts(self, kv_heads: int, size: int):
         """(parts, steps of a part) of the dK / dV pass: a block walks over every query that sees its keys - 16384 queries of 8 heads are 4096
         steps -, so a tile's steps are cut where one chain would be longer than the device's share of all of them."""
-        piece = max(PART_MIN, -(-self.key_work * kv_heads // FILL_BLOCKS))
-        if self.key_most <= piece:
+        piece = max(PART_MIN[size], -(-self.key_work * kv_heads // FILL_BLOCKS))
+        if self.key_most <= piece or self.key_most < 2 * PART_MIN[size]:
             return 1, 0
         return -(-self.key_most // piece), piece
 

@@ -5,7 +5,7 @@ import torch
 
 from crog_amd import _lib
 from crog_amd import functional as Fn
-from crog_amd.packed import KEY_TILE, SPLIT_MIN, TILE, PackedRows, RotaryAxes
+from crog_amd.packed import KEY_TILE, PART_MIN, SPLIT_MIN, TILE, PackedRows, RotaryAxes
 
 
 def tables(p):
@@ -36,31 +36,33 @@ def test_plan_covers_every_row_and_key_once(causal, group):
 def test_plan_of_nothing():
     for lens in ([], [0], [0, 0]):
         p = PackedRows(lens, device="cpu")
-        assert (p.rows_q, p.n_row_tiles, p.n_key_tiles) == (0, 0, 0) and p.splits(8)[0] == 1
+        assert (p.rows_q, p.n_row_tiles, p.n_key_tiles) == (0, 0, 0) and p.splits(8, 2)[0] == 1 and p.parts(8, 2)[0] == 1
 
 
+@pytest.mark.parametrize("size", [2, 4])
 @pytest.mark.parametrize("seqs,keys,kv", [(1, 8192, 1), (1, 8192, 8), (16, 777, 8), (3, 65, 2), (600, 5000, 1), (1, 100000, 1)])
-def test_splits_cover_the_keys(seqs, keys, kv):
+def test_splits_cover_the_keys(seqs, keys, kv, size):
     p = PackedRows([1] * seqs, [keys] * seqs, device="cpu")
-    n, piece = p.splits(kv)
+    n, piece = p.splits(kv, size)
     if n == 1:
-        assert seqs * kv >= 512 or keys <= SPLIT_MIN
+        assert seqs * kv >= 512 or keys < 2 * SPLIT_MIN[size]
     else:
-        assert piece % 64 == 0 and n * piece >= keys > (n - 1) * piece and piece >= SPLIT_MIN // 2
+        assert piece % 64 == 0 and n * piece >= keys > (n - 1) * piece and piece >= SPLIT_MIN[size] // 2
 
 
+@pytest.mark.parametrize("size", [2, 4])
 @pytest.mark.parametrize("lq,lk,group,kv,causal", [([5000, 300], None, 4, 4, True), ([4096], None, 8, 1, True), ([16384], [20], 1, 8, False), ([20] * 32, None, 1, 8, True),
                                                    ([3000], [100], 2, 1, True)])
-def test_parts_cover_the_rows(lq, lk, group, kv, causal):
+def test_parts_cover_the_rows(lq, lk, group, kv, causal, size):
     p = PackedRows(lq, lk, group=group, causal=causal, device="cpu")
-    n, piece = p.parts(kv)
+    n, piece = p.parts(kv, size)
     # the steps of a sequence's first key, seen by all its queries but those that see nothing
     most = max((-(-q // 32) - max(0, q - k) * causal // 32) * group for q, k in zip(lq, lk or lq))
     assert p.key_most == most
     if n == 1:
-        assert most <= max(32, -(-p.key_work * kv // 512))
+        assert most < 2 * PART_MIN[size] or most <= -(-p.key_work * kv // 512)
     else:
-        assert piece >= 32 and n * piece >= most > (n - 1) * piece
+        assert piece >= PART_MIN[size] and n * piece >= most > (n - 1) * piece
 
 
 @pytest.mark.parametrize("make,error", [
@@ -158,8 +160,8 @@ def test_c_entries_refuse_before_any_launch():
     for kw in bad:
         assert fwd(**kw) == -1, kw
         assert b"packed_attn_fwd" in lib.crog_last_error()
-    args = [1] + [p, 64, 64] * 5 + [p, p] + [p, 64, 64] * 3 + [p, p, p, 1, p, 1, 1, 8, 8, 1, 1, 64, 1.0, 0, 1, 0, None, None]
-    for at, v in ((0, 2), (1, None), (13, p + 8), (16, None), (17, None), (20, 4), (27, None), (38, 60), (41, 2), (41, 0), (2, 1 << 40), (5, 1 << 30)):
+    args = [1] + [p, 64, 64] * 5 + [p, p] + [p, 64, 64] * 3 + [p, p, p, 1, p, 1, 1, 8, 8, 1, 1, 64, 1.0, 0, 1, 0, 1, 0, None, None]
+    for at, v in ((0, 2), (1, None), (13, p + 8), (16, None), (17, None), (20, 4), (27, None), (38, 60), (41, 2), (41, 0), (43, 2), (43, 0), (2, 1 << 40), (5, 1 << 30)):
         assert lib.crog_packed_attn_bwd(*args[:at], v, *args[at + 1:]) == -1, at
     r = [1, p, 64, 64, p, 64, 64, p, 64, 64, p, 64, 64, p, 1, 4, p, p, 8, 1, 1, 64, 32, 1, 0, 0, None]
     for at, v in ((0, 2), (1, None), (13, None), (14, 0), (15, 2), (16, None), (18, -1), (22, 33), (22, 0), (23, 0)):
