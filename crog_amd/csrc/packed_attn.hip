@@ -20,6 +20,7 @@ constexpr int NT = 256;      // 4 waves
 constexpr int BR = 128;      // rows of a block (forward, dQ)
 constexpr int BK = 128;      // keys of a block (dK / dV)
 constexpr int RT = 32;       // query rows of a dK / dV step
+constexpr int OPERANDS = 2;      // what a dK / dV tile's operands and results count, in steps
 
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 
@@ -29,8 +30,8 @@ struct PackedArgs {
   float *lse, *D;      // [heads][rows_q], lse in log2 units (+inf: no key, so that 2^(s - lse) is 0)
   float *part_o, *part_ml;
   long ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso, lddo, hsdo, lddq, hsdq, lddk, hsdk, lddv, hsdv;
-  const int *cu_q, *cu_k, *tiles;
-  int seqs, rows_q, rows_k, kv_heads, group, dim, causal, split_keys, piece, parts;
+  const int *cu_q, *cu_k, *tiles, *units;
+  int seqs, rows_q, rows_k, kv_heads, group, dim, causal, split_keys, n_tiles, share;
   float scale;
 };
 
@@ -604,170 +605,218 @@ __global__ void __launch_bounds__(NT) packed_dq_sum_kernel(const PackedArgs a, i
 }
 
 // =====================================================================================================================
-// backward 2: dK, dV.  grid (kv_heads * key tiles, parts); a block owns 128 keys, 32 a wave, and the group's query rows stream past them through a
-// ring of four LDS tiles of 32 rows, requested three steps ahead.  Measured on the way (six causal sequences of up to 5000 rows, 16 / 4 heads of 128,
-// dK / dV alone): 128 keys, one chain of all rows a block, registers spilled 3910 us; rows straight into LDS 2200; 64 keys and two halves of the
-// rows a block, no spills 815; blocks that read the same rows at the same time 694 (of which a quarter waited for the next tile).
-// A key tile with more than `piece` steps is cut into parts, a block each, whose float sums meet in packed_parts_kernel in order.
-// =====================================================================================================================
-struct Parts { int begin, end, n; };
+// backward 2: dK, dV.  A block takes 128 keys at a time, 32 a wave, and the group's query rows stream past them through a ring of four LDS tiles of
+// 32 rows, requested three steps ahead.
 // A key tile's steps are 32 queries (of a grid from the sequence's first) of one head each, from the LAST queries backwards, the group's heads
-// inside: every key tile of a sequence starts with the same step, so the blocks of one key head read the same rows at the same time.  (From the
-// first query that sees the tile, head by head, half of these reads missed the L2: 2.7 GB from beyond it in the case above.)
-// Steps [begin, end) of part y, and the number of parts.
-__device__ inline Parts parts_of(const PackedArgs& a, const Seq& e, int tile, int y) {
-  Parts p;
+// inside: every key tile of a sequence starts with the same step.
+// The steps of all tiles lie one behind the other on one axis, each tile's with OPERANDS units more for its operands and results, and every block takes an
+// equal share of that axis (share > 0): causal or ragged tiles have anything between one step and thousands, and in pieces of equal length left CUs
+// idle for a quarter of the time (six causal sequences of up to 5000 rows, 16 / 4 heads of 128: 796 + 16 us to meet, in shares 638 + 26, 0.98
+// PFLOP/s; where every block has as many steps in any case 1.1 PFLOP/s).  A tile that lies in several shares leaves a float sum in each, two places a block, which meet in
+// packed_meet_kernel in order.  share 0: a block a tile.
+// =====================================================================================================================
+__device__ inline int steps_of(const PackedArgs& a, const Seq& e, int tile) {
   const int first = a.causal ? min(max(tile * BK - (e.lk - e.lq), 0), e.lq) : 0;
-  const int steps = ((e.lq + RT - 1) / RT - first / RT) * a.group;
-  p.n = min(max((int)(((long)steps + a.piece - 1) / a.piece), 1), a.parts);
-  p.begin = (int)min((long)y * a.piece, (long)steps);
-  p.end = y == p.n - 1 ? steps : (int)min((long)p.begin + a.piece, (long)steps);
-  return p;
+  return ((e.lq + RT - 1) / RT - first / RT) * a.group;
+}
+
+// the kernel's argument, loaded where it is used again: kept in registers through a loop of segments, its 60 words did not fit beside the loop's own
+__device__ inline PackedArgs args_again() {
+#ifdef __HIP_DEVICE_COMPILE__
+  auto p = (const __attribute__((address_space(4))) PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *p;
+#else
+  return {};      // (the host's pass has no address spaces)
+#endif
 }
 
 template <typename T, int DP, int DC>
-__global__ void __launch_bounds__(NT, sizeof(T) == 2 ? 2 : 1) packed_bwd_dkdv_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(NT, sizeof(T) == 2 ? DC <= 32 ? 4 : DC <= 64 ? 3 : 2 : 1) packed_bwd_dkdv_kernel(const PackedArgs args) {
   using L = Tile<T, DP, DC>;
   using F = Fetch<T, DP, RT>;
   constexpr int RING = 4, REQ = 2 * F::NR + 2;      // tiles of the ring, requests of a wave and step
   __shared__ __attribute__((aligned(16))) T sQ[RING][RT * DP];
   __shared__ __attribute__((aligned(16))) T sG[RING][RT * DP];
   __shared__ __attribute__((aligned(16))) float sS[RING][4][2][64];      // every wave fetches its own lse and D (32 of the 64): all have as many requests
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, ln = lane & 31;
-  const int kh = blockIdx.x % a.kv_heads, ti = blockIdx.x / a.kv_heads;
-  const int tile = a.tiles[2 * ti + 1];
-  const Seq e = seq_of(a, a.tiles[2 * ti]);
-  const int dim = a.dim;
-  if (tile < 0 || (long)tile * BK >= e.lk) return;      // (uniform)
-  const int k0 = tile * BK + wave * 32, key = k0 + ln, kc = min(key, e.lk - 1);
-  const Parts part = parts_of(a, e, tile, blockIdx.y);
-  if ((int)blockIdx.y >= part.n) return;      // (uniform)
-  const int off = e.lk - e.lq;
-  const int qmin = a.causal ? key - off : 0;      // the lane's key is seen by queries >= qmin
-  const int wbeg = a.causal ? k0 - off : 0, wall = a.causal ? k0 + 31 - off : 0;      // the wave's first query at all, its first that sees all its keys
-  const long hd0 = (long)kh * a.group;
-
-  Vec16<T> kf[L::NS], vf[L::NS];
-  load_frag<T, DP, DC>(kf, (const T*)a.K + (long)(e.k0 + kc) * a.ldk + (long)kh * a.hsk, h, dim, key < e.lk);
-  load_frag<T, DP, DC>(vf, (const T*)a.V + (long)(e.k0 + kc) * a.ldv + (long)kh * a.hsv, h, dim, key < e.lk);
-  f32x16 dk[L::NC], dv[L::NC];
-#pragma unroll
-  for (int c = 0; c < L::NC; c++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) dk[c][i] = dv[c][i] = 0.f;
-  const float c2 = a.scale * LOG2E;
-  F fq, fg;
-  fq.init(wave, lane, a.ldq);
-  fg.init(wave, lane, a.lddo);
-  const unsigned lds_q = lds_of(sQ), lds_g = lds_of(sG), lds_s = lds_of(sS) + wave * 2 * 64 * 4;
-  const int rows_at = L::rows_at(lane), cols_at = L::cols_at(lane);
-
-  // the next step to be requested: its head and first query, and running pointers to its rows
-  int hd = part.begin % a.group, q = ((e.lq + RT - 1) / RT - 1 - part.begin / a.group) * RT;
-  const T* qp = (const T*)a.Q + (long)(e.q0 + q) * a.ldq + (hd0 + hd) * a.hsq;
-  const T* gp = (const T*)a.dO + (long)(e.q0 + q) * a.lddo + (hd0 + hd) * a.hsdo;
-  const float *lp = a.lse + (hd0 + hd) * a.rows_q + e.q0 + q, *Dp = a.D + (hd0 + hd) * a.rows_q + e.q0 + q;
-  const long next_q = RT * a.ldq + (a.group - 1) * a.hsq, next_g = RT * a.lddo + (a.group - 1) * a.hsdo, next_s = RT + (a.group - 1) * (long)a.rows_q;
-  const auto request = [&](int slot) {      // (rows that do not exist are zeros throughout: their dS is 0 and their dO is)
-    fq.get(lds_q + slot * RT * L::RB, qp, e.lq - q, dim);
-    fg.get(lds_g + slot * RT * L::RB, gp, e.lq - q, dim);
-    const unsigned so = lane < RT && q + lane < e.lq ? lane * 4 : DMA_OOB;
-    dma_word_at(lp, lds_s + slot * 4 * 2 * 64 * 4, so);
-    dma_word_at(Dp, lds_s + slot * 4 * 2 * 64 * 4 + 64 * 4, so);
-    if (++hd < a.group) {
-      qp += a.hsq;
-      gp += a.hsdo;
-      lp += a.rows_q;
-      Dp += a.rows_q;
-    } else {      // the first head of the queries before
-      hd = 0;
-      q -= RT;
-      qp -= next_q;
-      gp -= next_g;
-      lp -= next_s;
-      Dp -= next_s;
+  int kh, ti, block = blockIdx.x;
+  long pos = 0, end = 1;
+  if (args.share == 0) {
+    kh = block % args.kv_heads;
+    ti = block / args.kv_heads;
+  } else {
+    // neighbouring shares on one XCD: they read the same rows (workgroups go round the 8 XCDs; the grid is a multiple of 8)
+    block = block % 8 * (gridDim.x / 8) + block / 8;
+    const long total = args.units[args.n_tiles];
+    pos = (long)block * args.share;
+    end = min(pos + args.share, total * args.kv_heads);
+    if (pos >= end) return;
+    kh = (int)(pos / total);
+    const int u = (int)(pos - kh * total);
+    int lo = 0, hi = args.n_tiles;      // units[lo] <= u < units[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (args.units[mid] <= u) lo = mid;
+      else hi = mid;
     }
-  };
-  wait_vmcnt<0>();      // (the operands above: from here on only requests are counted)
-  const int steps = part.end - part.begin;
-#pragma unroll
-  for (int i = 0; i < RING - 1; i++)
-    if (i < steps) request(i);
-  int hd_now = part.begin % a.group, q_now = ((e.lq + RT - 1) / RT - 1 - part.begin / a.group) * RT;
-  for (int st = 0; st < steps; st++) {
-    // this step's tile is there, and (the barrier) every wave is done with the one before, whose place the step three ahead takes
-    if (st + 2 < steps) wait_vmcnt<2 * REQ>();
-    else if (st + 1 < steps) wait_vmcnt<REQ>();
-    else wait_vmcnt<0>();
-    __syncthreads();
-    if (st + RING - 1 < steps) request((st + RING - 1) % RING);
-    const int r0 = q_now;
-    if (++hd_now == a.group) {
-      hd_now = 0;
-      q_now -= RT;
-    }
-    if (k0 >= e.lk || r0 + RT <= wbeg) continue;
-    const int buf = st % RING;
-    int at_r = rows_at + buf * RT * L::RB, at_c = cols_at + buf * RT * L::RB;
-    opaque(at_r);
-    opaque(at_c);
-    f32x16 s, dp;
-#pragma unroll
-    for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
-    __builtin_amdgcn_s_setprio(1);      // (products first: where the waves of a SIMD meet in the same phase, backward 218 -> 200 us at 676 tokens)
-    mma_rows<T, DP, DC>(s, sQ[0], at_r, 0, kf);
-    mma_rows<T, DP, DC>(dp, sG[0], at_r, 0, vf);
-    __builtin_amdgcn_s_setprio(0);
-    if (r0 < wall)
-#pragma unroll
-      for (int i = 0; i < 16; i++) s[i] = r0 + acc_row(i, h) >= qmin ? s[i] * c2 : -INFINITY;
-    else
-#pragma unroll
-      for (int i = 0; i < 16; i++) s[i] *= c2;
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const f32x4 l4 = *reinterpret_cast<const f32x4*>(&sS[buf][wave][0][8 * g + 4 * h]), d4 = *reinterpret_cast<const f32x4*>(&sS[buf][wave][1][8 * g + 4 * h]);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int i = 4 * g + j;
-        s[i] = ex2(s[i] - l4[j]);
-        dp[i] = s[i] * (dp[i] - d4[j]);      // (the scale follows at the end)
+    ti = lo;
+  }
+  while (pos < end) {
+    const PackedArgs a = args_again();
+    int tid = threadIdx.x;
+    opaque(tid);      // (what depends on the lane alone is formed again for each segment too)
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, ln = lane & 31;
+    const int dim = a.dim;
+    const int tile = a.tiles[2 * ti + 1];
+    const Seq e = seq_of(a, a.tiles[2 * ti]);
+    const int all = steps_of(a, e, tile);
+    int first = 0, last = all, slot = -1;      // steps of this segment; place of its float sum (-1: the whole tile)
+    const int hn = kh;
+    if (a.share == 0) {
+      pos = end;
+    } else {
+      const long at = (long)kh * a.units[a.n_tiles] + a.units[ti];
+      const int mine = a.units[ti + 1] - a.units[ti];
+      const int u0 = (int)min(max(pos - at, 0l), (long)mine), u1 = (int)min(end - at, (long)mine);
+      if (u0 > 0 || u1 < mine) slot = 2 * block + (u0 == 0);
+      first = min(max(u0 - OPERANDS, 0), all);
+      last = u1 == mine ? all : min(max(u1 - OPERANDS, first), all);
+      pos = max(pos + 1, at + mine);      // (on, whatever the table holds)
+      if (++ti == a.n_tiles) {
+        ti = 0;
+        kh = min(kh + 1, a.kv_heads - 1);
       }
     }
-    __builtin_amdgcn_s_setprio(1);
-    mma_cols<T, DP, DC>(dv, sG[0], at_c, 0, s);
-    mma_cols<T, DP, DC>(dk, sQ[0], at_c, 0, dp);
-    __builtin_amdgcn_s_setprio(0);
+    if (tile < 0 || (long)tile * BK >= e.lk) continue;      // (uniform)
+    const int k0 = tile * BK + wave * 32, key = k0 + ln, kc = min(key, e.lk - 1);
+    const int off = e.lk - e.lq;
+    const int qmin = a.causal ? key - off : 0;      // the lane's key is seen by queries >= qmin
+    const int wbeg = a.causal ? k0 - off : 0, wall = a.causal ? k0 + 31 - off : 0;      // the wave's first query at all, its first that sees all its keys
+    const long hd0 = (long)hn * a.group;
+
+    Vec16<T> kf[L::NS], vf[L::NS];
+    load_frag<T, DP, DC>(kf, (const T*)a.K + (long)(e.k0 + kc) * a.ldk + (long)hn * a.hsk, h, dim, key < e.lk);
+    load_frag<T, DP, DC>(vf, (const T*)a.V + (long)(e.k0 + kc) * a.ldv + (long)hn * a.hsv, h, dim, key < e.lk);
+    f32x16 dk[L::NC], dv[L::NC];
+#pragma unroll
+    for (int c = 0; c < L::NC; c++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) dk[c][i] = dv[c][i] = 0.f;
+    const float c2 = a.scale * LOG2E;
+    F fq, fg;
+    fq.init(wave, lane, a.ldq);
+    fg.init(wave, lane, a.lddo);
+    const unsigned lds_q = lds_of(sQ), lds_g = lds_of(sG), lds_s = lds_of(sS) + wave * 2 * 64 * 4;
+    const int rows_at = L::rows_at(lane), cols_at = L::cols_at(lane);
+
+    // the next step to be requested: its head and first query, and running pointers to its rows
+    int hd = first % a.group, q = ((e.lq + RT - 1) / RT - 1 - first / a.group) * RT;
+    const T* qp = (const T*)a.Q + (long)(e.q0 + q) * a.ldq + (hd0 + hd) * a.hsq;
+    const T* gp = (const T*)a.dO + (long)(e.q0 + q) * a.lddo + (hd0 + hd) * a.hsdo;
+    const float *lp = a.lse + (hd0 + hd) * a.rows_q + e.q0 + q, *Dp = a.D + (hd0 + hd) * a.rows_q + e.q0 + q;
+    const long next_q = RT * a.ldq + (a.group - 1) * a.hsq, next_g = RT * a.lddo + (a.group - 1) * a.hsdo, next_s = RT + (a.group - 1) * (long)a.rows_q;
+    const auto request = [&](int slot) {      // (rows that do not exist are zeros throughout: their dS is 0 and their dO is)
+      fq.get(lds_q + slot * RT * L::RB, qp, e.lq - q, dim);
+      fg.get(lds_g + slot * RT * L::RB, gp, e.lq - q, dim);
+      const unsigned so = lane < RT && q + lane < e.lq ? lane * 4 : DMA_OOB;
+      dma_word_at(lp, lds_s + slot * 4 * 2 * 64 * 4, so);
+      dma_word_at(Dp, lds_s + slot * 4 * 2 * 64 * 4 + 64 * 4, so);
+      if (++hd < a.group) {
+        qp += a.hsq;
+        gp += a.hsdo;
+        lp += a.rows_q;
+        Dp += a.rows_q;
+      } else {      // the first head of the queries before
+        hd = 0;
+        q -= RT;
+        qp -= next_q;
+        gp -= next_g;
+        lp -= next_s;
+        Dp -= next_s;
+      }
+    };
+    wait_vmcnt<0>();      // (the operands above: from here on only requests are counted)
+    __syncthreads();      // (every wave is done with the segment before)
+    const int steps = last - first;
+#pragma unroll
+    for (int i = 0; i < RING - 1; i++)
+      if (i < steps) request(i);
+    int hd_now = first % a.group, q_now = ((e.lq + RT - 1) / RT - 1 - first / a.group) * RT;
+    for (int st = 0; st < steps; st++) {
+      // this step's tile is there, and (the barrier) every wave is done with the one before, whose place the step three ahead takes
+      if (st + 2 < steps) wait_vmcnt<2 * REQ>();
+      else if (st + 1 < steps) wait_vmcnt<REQ>();
+      else wait_vmcnt<0>();
+      __syncthreads();
+      if (st + RING - 1 < steps) request((st + RING - 1) % RING);
+      const int r0 = q_now;
+      if (++hd_now == a.group) {
+        hd_now = 0;
+        q_now -= RT;
+      }
+      if (k0 >= e.lk || r0 + RT <= wbeg) continue;
+      const int buf = st % RING;
+      int at_r = rows_at + buf * RT * L::RB, at_c = cols_at + buf * RT * L::RB;
+      opaque(at_r);
+      opaque(at_c);
+      f32x16 s, dp;
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
+      __builtin_amdgcn_s_setprio(1);      // (products first, where the waves of a SIMD compete: 32 sequences of 676 tokens, a training pass 246 -> 221 us)
+      mma_rows<T, DP, DC>(s, sQ[0], at_r, 0, kf);
+      mma_rows<T, DP, DC>(dp, sG[0], at_r, 0, vf);
+      __builtin_amdgcn_s_setprio(0);
+      if (r0 < wall)
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = r0 + acc_row(i, h) >= qmin ? s[i] * c2 : -INFINITY;
+      else
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] *= c2;
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const f32x4 l4 = *reinterpret_cast<const f32x4*>(&sS[buf][wave][0][8 * g + 4 * h]);
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&sS[buf][wave][1][8 * g + 4 * h]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int i = 4 * g + j;
+          s[i] = ex2(s[i] - l4[j]);
+          dp[i] = s[i] * (dp[i] - d4[j]);      // (the scale follows at the end)
+        }
+      }
+      __builtin_amdgcn_s_setprio(1);
+      mma_cols<T, DP, DC>(dv, sG[0], at_c, 0, s);
+      mma_cols<T, DP, DC>(dk, sQ[0], at_c, 0, dp);
+      __builtin_amdgcn_s_setprio(0);
+    }
+    if (key < e.lk && slot >= 0) {
+      float* p = a.part_o + ((long)slot * BK + wave * 32 + ln) * 2 * dim;
+      store_row<float, DC>(p, dk, h, dim, a.scale);
+      store_row<float, DC>(p + dim, dv, h, dim, 1.f);
+    } else if (key < e.lk) {
+      store_row<T, DC>((T*)a.dK + (long)(e.k0 + key) * a.lddk + (long)hn * a.hsdk, dk, h, dim, a.scale);
+      store_row<T, DC>((T*)a.dV + (long)(e.k0 + key) * a.lddv + (long)hn * a.hsdv, dv, h, dim, 1.f);
+    }
   }
-  if (key >= e.lk) return;
-  if (part.n > 1) {
-    float* p = a.part_o + (((long)blockIdx.y * a.kv_heads + kh) * a.rows_k + e.k0 + key) * 2 * dim;
-    store_row<float, DC>(p, dk, h, dim, a.scale);
-    store_row<float, DC>(p + dim, dv, h, dim, 1.f);
-    return;
-  }
-  store_row<T, DC>((T*)a.dK + (long)(e.k0 + key) * a.lddk + (long)kh * a.hsdk, dk, h, dim, a.scale);
-  store_row<T, DC>((T*)a.dV + (long)(e.k0 + key) * a.lddv + (long)kh * a.hsdv, dv, h, dim, 1.f);
 }
 
-// dK, dV of the key tiles in several parts, summed in order.  grid (kv_heads * key tiles, chunks of 16 keys)
+// dK, dV of the key tiles in several shares, summed in order.  grid (kv_heads * key tiles, chunks of 16 keys)
 template <typename T>
-__global__ void __launch_bounds__(NT) packed_parts_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(NT) packed_meet_kernel(const PackedArgs a, int blocks) {
   const int kh = blockIdx.x % a.kv_heads, ti = blockIdx.x / a.kv_heads;
   const int tile = a.tiles[2 * ti + 1];
   const Seq e = seq_of(a, a.tiles[2 * ti]);
   if (tile < 0 || (long)tile * BK + blockIdx.y * 16 >= e.lk) return;
-  const int k0 = tile * BK + blockIdx.y * 16;
-  const int n = parts_of(a, e, tile, 0).n;
-  if (n == 1) return;
-  const int keys = min(16, e.lk - k0), per = 2 * a.dim / 4;
-  const long step = (long)a.kv_heads * a.rows_k * 2 * a.dim;
+  const long at = (long)kh * a.units[a.n_tiles];
+  const int b0 = (int)min((at + a.units[ti]) / a.share, (long)blocks - 1), b1 = (int)min((at + a.units[ti + 1] - 1) / a.share, (long)blocks - 1);
+  if (b0 >= b1 || b0 < 0) return;
+  const int k0 = blockIdx.y * 16, keys = min(16, e.lk - tile * BK - k0), per = 2 * a.dim / 4;
   for (int i = threadIdx.x; i < keys * per; i += NT) {
-    const int k = i / per, c = (i - k * per) * 4;
-    const long key = e.k0 + k0 + k;
-    const float* from = a.part_o + ((long)kh * a.rows_k + key) * 2 * a.dim + c;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int y = 0; y < n; y++) v += *reinterpret_cast<const f32x4*>(from + y * step);
+    const int k = k0 + i / per, c = (i % per) * 4;
+    const auto sum_of = [&](int slot) { return *reinterpret_cast<const f32x4*>(a.part_o + ((long)slot * BK + k) * 2 * a.dim + c); };
+    f32x4 v = sum_of(2 * b0 + 1);
+#pragma unroll 4
+    for (int b = b0 + 1; b <= b1; b++) v += sum_of(2 * b);
+    const long key = e.k0 + tile * BK + k;
     T* p = c < a.dim ? (T*)a.dK + key * a.lddk + (long)kh * a.hsdk + c : (T*)a.dV + key * a.lddv + (long)kh * a.hsdv + c - a.dim;
 #pragma unroll
     for (int j = 0; j < 4; j++) p[j] = Elem<T>::from_f(v[j]);
@@ -847,7 +896,8 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
                                     const float* lse, float* D, void* dQ, int64_t lddq, int64_t hsdq, void* dK, int64_t lddk, int64_t hsdk, void* dV,
                                     int64_t lddv, int64_t hsdv, const int* cu_q, const int* cu_k, const int* row_tiles, int n_row_tiles,
                                     const int* key_tiles, int n_key_tiles, int seqs, int rows_q, int rows_k, int kv_heads, int group, int head_dim,
-                                    float scale, int causal, int splits, int split_keys, int parts, int part_steps, float* partial, crog_stream_t stream) {
+                                    float scale, int causal, int splits, int split_keys, const int* key_units,
+                                    int total_units, int share, float* partial, crog_stream_t stream) {
   if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_row_tiles, cu_q, cu_k, row_tiles)) return rc;
   if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_key_tiles, cu_q, cu_k, key_tiles)) return rc;
   const int vec = dtype == CROG_BF16 ? 8 : 4;
@@ -856,8 +906,8 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
                  "packed_attn_bwd: heads of Q / K / V / O / dO and the gradients must start at 16-byte boundaries");
   CROG_CHECK_ARG(splits >= 1 && splits <= 65535 && (splits == 1 || (partial && split_keys > 0 && split_keys % 64 == 0)),
                  "packed_attn_bwd: %d splits need a workspace and a multiple of 64 keys each (got %d)", splits, split_keys);
-  CROG_CHECK_ARG(parts >= 1 && parts <= 65535 && (parts == 1 || (part_steps > 0 && partial)),
-                 "packed_attn_bwd: %d parts need a workspace and a number of steps each (got %d)", parts, part_steps);
+  CROG_CHECK_ARG(share >= 0 && (share == 0 || (key_units && total_units >= n_key_tiles && partial && cdiv((int64_t)total_units * kv_heads, share) < (1 << 24))),
+                 "packed_attn_bwd: shares of %d units need their table (%d units) and a workspace", share, total_units);
   CROG_CHECK_ARG(near(ldk, dtype) && near(ldv, dtype) && near(ldq, dtype) && near(lddo, dtype),
                  "packed_attn_bwd: 64 rows must lie within 2 GiB");
   PackedArgs a{};
@@ -886,15 +936,17 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
   }
   if (n_key_tiles > 0) {
     a.tiles = key_tiles;
-    a.parts = parts;
-    a.piece = parts > 1 ? part_steps : 0x7fffff00;
+    a.n_tiles = n_key_tiles;
+    a.units = key_units;
+    a.share = share;
     a.part_o = partial;
-    const dim3 n((unsigned)(n_key_tiles * kv_heads), parts);
-    for_dim(dtype, head_dim, [&](auto t, auto dp, auto dc) { packed_bwd_dkdv_kernel<decltype(t), dp(), dc()><<<n, NT, 0, s>>>(a); });
+    const unsigned n = (unsigned)(n_key_tiles * kv_heads), blocks = share > 0 ? (unsigned)cdiv((int64_t)total_units * kv_heads, share) : n;
+    const unsigned grid = share > 0 ? (blocks + 7) / 8 * 8 : n;
+    for_dim(dtype, head_dim, [&](auto t, auto dp, auto dc) { packed_bwd_dkdv_kernel<decltype(t), dp(), dc()><<<grid, NT, 0, s>>>(a); });
     CROG_LAUNCH_CHECK();
-    if (parts > 1) {
-      if (dtype == CROG_BF16) packed_parts_kernel<bf16><<<dim3(n.x, BK / 16), NT, 0, s>>>(a);
-      else packed_parts_kernel<float><<<dim3(n.x, BK / 16), NT, 0, s>>>(a);
+    if (share > 0) {
+      if (dtype == CROG_BF16) packed_meet_kernel<bf16><<<dim3(n, BK / 16), NT, 0, s>>>(a, (int)blocks);
+      else packed_meet_kernel<float><<<dim3(n, BK / 16), NT, 0, s>>>(a, (int)blocks);
       CROG_LAUNCH_CHECK();
     }
   }

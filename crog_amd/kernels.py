@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import GemmDesc, check as _check
+from .packed import KEY_TILE
 
 F32, BF16 = 0, 1
 A_KC, A_IM2COL, A_MC = 0, 1, 2
@@ -796,14 +797,14 @@ def packed_attn_fwd(q, k, v, o, lse, rows, scale):
 def packed_attn_bwd(q, k, v, o, do, lse, D, dq, dk, dv, rows, scale):
     _, kv, dim = k.shape
     size = q.element_size()
-    (splits, keys), (parts, steps) = rows.splits(kv, size), rows.parts(kv, size)
+    (splits, keys), (share, blocks) = rows.splits(kv, size), rows.share(kv, dim, size)
     plan_used(rows)
-    floats = max(splits * kv * rows.group * rows.rows_q * dim if splits > 1 else 0, parts * kv * rows.rows_k * 2 * dim if parts > 1 else 0)
+    floats = max(splits * kv * rows.group * rows.rows_q * dim if splits > 1 else 0, blocks * 2 * KEY_TILE * 2 * dim if share else 0)
     ws = torch.empty(floats, device=q.device, dtype=torch.float32) if floats else None
     check(lib().crog_packed_attn_bwd(dcode(q), *_heads(q), *_heads(k), *_heads(v), *_heads(o), *_heads(do), ptr(lse), ptr(D), *_heads(dq), *_heads(dk),
                                      *_heads(dv), rows.cu_q_ptr, rows.cu_k_ptr, rows.row_tiles_ptr, rows.n_row_tiles, rows.key_tiles_ptr,
-                                     rows.n_key_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, splits, keys, parts, steps,
-                                     ptr(ws), stream()), "packed_attn_bwd")
+                                     rows.n_key_tiles, rows.seqs, rows.rows_q, rows.rows_k, kv, rows.group, dim, scale, rows.causal, splits, keys,
+                                     rows.key_units_ptr, rows.key_units, share, ptr(ws), stream()), "packed_attn_bwd")
 
 
 def rotary(q, k, q_out, k_out, positions, axes, inverse=False):

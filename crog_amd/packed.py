@@ -14,14 +14,17 @@ import torch
 
 TILE = 128      # rows (query rows x heads of a group) of a forward / dQ block of csrc/packed_attn.hip
 KEY_TILE = 128  # keys of a dK / dV block
-# Long chains of work are cut where there are too few blocks to fill the device (256 CUs, two blocks each): the keys that a block of the forward or
-# dQ pass walks over, the queries that a block of the dK / dV pass walks over.  The pieces meet in a second launch, which costs 4 to 8 us, so a piece
-# has at least SPLIT_MIN keys or PART_MIN steps (by the bytes of an element; fp32 products take eight times as long).  100 keys over 4000 queries of 8
-# heads, bf16: dK / dV 27 us in one part, 17 + 4 in two; one token over 8192 keys, 8 key heads: 85 us in one piece, 11 + 6 in 32.  Twice, four times
-# and eight times as many blocks were no faster or slower.
+# Long chains of work are cut where there are too few blocks to fill the device (256 CUs, two blocks each) or where it would wait for the longest: the
+# keys that a block of the forward or dQ pass walks over in equal pieces, the steps of the dK / dV pass in equal shares of all of them.  The pieces meet
+# in a second launch, which costs 4 to 25 us, so a piece has at least SPLIT_MIN keys or SHARE_MIN units (by the bytes of an element; fp32 products take
+# eight times as long).  100 keys over 4000 queries of 8 heads, bf16: dK / dV 27 us uncut, 16 + 4 cut; one token over 8192 keys, 8 key heads: 85 us in
+# one piece, 11 + 6 in 32; two, four and eight times as many pieces were no faster or slower.
 FILL_BLOCKS = 512
 SPLIT_MIN = {2: 256, 4: 128}
-STEP, PART_MIN = 32, {2: 8, 4: 4}      # queries of a dK / dV step
+# dK / dV: blocks that the device holds, by head_dim / 32 (bf16; fp32: one a CU); queries of a step; units of a tile's operands and results; units of a
+# share at least.
+SLOTS, SLOTS_FP32 = {1: 1024, 2: 768, 3: 512, 4: 512}, 256
+STEP, OPERANDS, SHARE_MIN = 32, 2, {2: 8, 4: 4}
 
 
 def _stream_of(table: torch.Tensor):
@@ -42,14 +45,14 @@ def _lengths(name: str, lengths: Sequence[int]) -> np.ndarray:
     return np.asarray(out, dtype=np.int64)
 
 
-def _tiles(rows: np.ndarray, size: int, cost):
-    """[(sequence, tile)] of all tiles of `size` rows, the costliest first (a late long one would leave the device waiting for a single block),
-    and their costs."""
+def _tiles(rows: np.ndarray, size: int, cost, together: bool = False):
+    """[(sequence, tile)] of all tiles of `size` rows and their costs, the costliest first (a late long one would leave the device waiting for a
+    single block); together: a sequence's tiles one behind the other, the sequence with the costliest first."""
     n = (rows + size - 1) // size
     seq = np.repeat(np.arange(len(rows)), n)
     tile = np.arange(len(seq)) - np.repeat(np.cumsum(n) - n, n)
     c = cost(seq, tile)
-    order = np.argsort(-c, kind="stable")
+    order = np.argsort(-(cost(seq, 0) if together else c), kind="stable")
     return np.stack([seq[order], tile[order]], 1), c[order]
 
 
@@ -85,11 +88,13 @@ class PackedRows:
             first = np.clip(t * KEY_TILE - (lk[s] - lq[s]), 0, lq[s]) if c else 0
             return ((lq[s] + STEP - 1) // STEP - first // STEP) * g
 
-        (rt, _), (kt, kc) = _tiles(lq * g, TILE, row_cost), _tiles(lk, KEY_TILE, key_cost)
-        self.key_work, self.key_most = int(kc.sum()), int(kc.max()) if len(kc) else 0
+        (rt, _), (kt, kc) = _tiles(lq * g, TILE, row_cost), _tiles(lk, KEY_TILE, key_cost, together=True)
+        kc = kc + OPERANDS
+        self.key_units, self.key_most = int(kc.sum()), int(kc.max()) if len(kc) else 0
         self.n_row_tiles, self.n_key_tiles = len(rt), len(kt)
         zero = np.zeros(1, dtype=np.int64)
-        parts = [np.concatenate([zero, np.cumsum(lq)]), np.concatenate([zero, np.cumsum(lk)]), rt.reshape(-1), kt.reshape(-1)]
+        parts = [np.concatenate([zero, np.cumsum(lq)]), np.concatenate([zero, np.cumsum(lk)]), rt.reshape(-1), kt.reshape(-1),
+                 np.concatenate([zero, np.cumsum(kc)]) if self.key_units < 1 << 31 else zero]
         table = torch.from_numpy(np.concatenate(parts).astype(np.int32))
         self._table = table.to(device)      # one copy; the tables lie in it one behind the other
         self.device, self.made_on = self._table.device, _stream_of(self._table)
@@ -97,7 +102,7 @@ class PackedRows:
         for p in parts:
             addr.append(self._table.data_ptr() + 4 * at)
             at += len(p)
-        self.cu_q_ptr, self.cu_k_ptr, self.row_tiles_ptr, self.key_tiles_ptr = addr
+        self.cu_q_ptr, self.cu_k_ptr, self.row_tiles_ptr, self.key_tiles_ptr, self.key_units_ptr = addr
 
     def splits(self, kv_heads: int, size: int):
         """(pieces, keys of a piece) of the forward and dQ passes' key axis; size: bytes of an element.  A single query over 8192 keys of 8 heads
@@ -110,13 +115,17 @@ class PackedRows:
         piece = -(-piece // 64) * 64
         return -(-self.max_k // piece), piece
 
-    def parts(self, kv_heads: int, size: int):
-        """(parts, steps of a part) of the dK / dV pass: a block walks over every query that sees its keys - 16384 queries of 8 heads are 4096
-        steps -, so a tile's steps are cut where one chain would be longer than the device's share of all of them."""
-        piece = max(PART_MIN[size], -(-self.key_work * kv_heads // FILL_BLOCKS))
-        if self.key_most <= piece or self.key_most < 2 * PART_MIN[size]:
-            return 1, 0
-        return -(-self.key_most // piece), piece
+    def share(self, kv_heads: int, dim: int, size: int):
+        """(units of a block, blocks) of the dK / dV pass: a block walks over every query that sees its keys - 16384 queries of 8 heads are 4096
+        steps -, so the steps of all tiles are dealt out evenly where the device would wait for the longest.  (0, blocks): a block a tile."""
+        slots = SLOTS[-(-dim // 32)] if size == 2 else SLOTS_FP32
+        n, work = self.n_key_tiles * kv_heads, self.key_units * kv_heads
+        even = max(-(-work // slots), SHARE_MIN[size])
+        # uncut: as long as the longest tile; with more tiles than places, half of it beyond an even share, or so many rounds of them
+        whole = max(self.key_most, min(even + self.key_most // 2, -(-n // slots) * self.key_most))
+        if whole <= even + SHARE_MIN[size] or self.key_units >= 1 << 31:
+            return 0, n
+        return even, -(-work // even)
 
 
 class RotaryAxes:

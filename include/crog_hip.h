@@ -619,9 +619,11 @@ int crog_preprocess_u8(const uint8_t* img, const uint8_t* masks, int B, int H, i
  * the backward, and scratch of the backward (rowsum(dO * O)).
  * splits > 1: the keys of a row are walked in `splits` pieces of split_keys (a multiple of 64; the last takes what is left) that meet in a second
  * launch; partial: splits * kv_heads * rows_q * group * (head_dim + 2) floats.
- * parts > 1: a key tile's steps - 32 queries of one head each, from the sequence's last back to the first that see it - are walked in up to `parts` pieces of part_steps (the
- * last takes what is left) that meet in a second launch; partial: the larger of parts * kv_heads * rows_k * 2 * head_dim floats and, for the splits
- * of dQ, splits * kv_heads * group * rows_q * head_dim.
+ * share > 0: a key tile's units - two, and one for each step of 32 queries (of a grid from the sequence's first) of one head that see it - lie
+ * behind those of the tiles before it in the list (key_units: device int32 table of n_key_tiles + 1 sums, from 0 to total_units), one key head's
+ * behind the other's, and each block walks `share` of them; a tile in several shares meets in a second launch.  0: a block a tile.
+ * partial: the larger of 2 * ceil(total_units * kv_heads / share) * 128 * 2 * head_dim floats and, for the splits of dQ,
+ * splits * kv_heads * group * rows_q * head_dim.
  * Rows outside every sequence are not read and not written.  Non-finite values of a key or value row may reach every query row of its own
  * sequence (also through a probability of zero), never another sequence; in the backward those of any row reach its sequence. */
 int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64_t hsq, const void* K, int64_t ldk, int64_t hsk,
@@ -634,7 +636,7 @@ int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64_t hsq, con
                          int64_t lddk, int64_t hsdk, void* dV, int64_t lddv, int64_t hsdv, const int* cu_q, const int* cu_k,
                          const int* row_tiles, int n_row_tiles, const int* key_tiles, int n_key_tiles, int seqs, int rows_q,
                          int rows_k, int kv_heads, int group, int head_dim, float scale, int causal, int splits, int split_keys,
-                         int parts, int part_steps, float* partial, crog_stream_t stream);
+                         const int* key_units, int total_units, int share, float* partial, crog_stream_t stream);
 /* Rotary positions: the first 2 * pairs (at most 256) columns of every head of Q (heads_q) and K (heads_k, may be 0) are pairs - column i with
  * column pairs + i, or, interleaved, 2 i with 2 i + 1 - that turn by positions[row * ldpos + axis[i]] * revs[i] revolutions (inverse: back);
  * the other columns are copied.  positions: int32 or int64 (pos_bytes 4 / 8); revs: `pairs` doubles, axis: `pairs` ints below `axes`, on the

@@ -5,14 +5,14 @@ import torch
 
 from crog_amd import _lib
 from crog_amd import functional as Fn
-from crog_amd.packed import KEY_TILE, PART_MIN, SPLIT_MIN, TILE, PackedRows, RotaryAxes
+from crog_amd.packed import KEY_TILE, OPERANDS, SHARE_MIN, SLOTS, SPLIT_MIN, TILE, PackedRows, RotaryAxes
 
 
 def tables(p):
     t = p._table.numpy()
     n = p.seqs + 1
     cu_q, cu_k, rest = t[:n], t[n:2 * n], t[2 * n:]
-    return cu_q, cu_k, rest[:2 * p.n_row_tiles].reshape(-1, 2), rest[2 * p.n_row_tiles:].reshape(-1, 2)
+    return cu_q, cu_k, rest[:2 * p.n_row_tiles].reshape(-1, 2), rest[2 * p.n_row_tiles:2 * (p.n_row_tiles + p.n_key_tiles)].reshape(-1, 2)
 
 
 @pytest.mark.parametrize("causal", [False, True])
@@ -36,7 +36,7 @@ def test_plan_covers_every_row_and_key_once(causal, group):
 def test_plan_of_nothing():
     for lens in ([], [0], [0, 0]):
         p = PackedRows(lens, device="cpu")
-        assert (p.rows_q, p.n_row_tiles, p.n_key_tiles) == (0, 0, 0) and p.splits(8, 2)[0] == 1 and p.parts(8, 2)[0] == 1
+        assert (p.rows_q, p.n_row_tiles, p.n_key_tiles) == (0, 0, 0) and p.splits(8, 2)[0] == 1 and p.share(8, 64, 2) == (0, 0)
 
 
 @pytest.mark.parametrize("size", [2, 4])
@@ -53,16 +53,24 @@ def test_splits_cover_the_keys(seqs, keys, kv, size):
 @pytest.mark.parametrize("size", [2, 4])
 @pytest.mark.parametrize("lq,lk,group,kv,causal", [([5000, 300], None, 4, 4, True), ([4096], None, 8, 1, True), ([16384], [20], 1, 8, False), ([20] * 32, None, 1, 8, True),
                                                    ([3000], [100], 2, 1, True)])
-def test_parts_cover_the_rows(lq, lk, group, kv, causal, size):
+def test_shares_cover_the_steps(lq, lk, group, kv, causal, size):
     p = PackedRows(lq, lk, group=group, causal=causal, device="cpu")
-    n, piece = p.parts(kv, size)
-    # the steps of a sequence's first key, seen by all its queries but those that see nothing
-    most = max((-(-q // 32) - max(0, q - k) * causal // 32) * group for q, k in zip(lq, lk or lq))
-    assert p.key_most == most
-    if n == 1:
-        assert most < 2 * PART_MIN[size] or most <= -(-p.key_work * kv // 512)
-    else:
-        assert piece >= PART_MIN[size] and n * piece >= most > (n - 1) * piece
+    # a tile's steps - 32 queries of one head - and OPERANDS units more, in the list's order
+    pairs, sums = tables(p)[3], p._table.numpy()[-p.n_key_tiles - 1:]
+    assert p.key_units_ptr == p.key_tiles_ptr + 8 * p.n_key_tiles
+    lks = lk or lq
+    want = []
+    for s, t in pairs.tolist():
+        first = min(max(t * KEY_TILE - (lks[s] - lq[s]), 0), lq[s]) if causal else 0
+        want.append((-(-lq[s] // 32) - first // 32) * group + OPERANDS)
+    assert sums[0] == 0 and np.diff(sums).tolist() == want and (p.key_units, p.key_most) == (sum(want), max(want))
+    for dim in (32, 64, 128):
+        share, blocks = p.share(kv, dim, size)
+        if share:
+            assert share >= SHARE_MIN[size] and share * blocks >= p.key_units * kv > share * (blocks - 1)
+            assert blocks <= SLOTS[dim // 32]
+        else:
+            assert blocks == p.n_key_tiles * kv
 
 
 @pytest.mark.parametrize("make,error", [
@@ -160,8 +168,8 @@ def test_c_entries_refuse_before_any_launch():
     for kw in bad:
         assert fwd(**kw) == -1, kw
         assert b"packed_attn_fwd" in lib.crog_last_error()
-    args = [1] + [p, 64, 64] * 5 + [p, p] + [p, 64, 64] * 3 + [p, p, p, 1, p, 1, 1, 8, 8, 1, 1, 64, 1.0, 0, 1, 0, 1, 0, None, None]
-    for at, v in ((0, 2), (1, None), (13, p + 8), (16, None), (17, None), (20, 4), (27, None), (38, 60), (41, 2), (41, 0), (43, 2), (43, 0), (2, 1 << 40), (5, 1 << 30)):
+    args = [1] + [p, 64, 64] * 5 + [p, p] + [p, 64, 64] * 3 + [p, p, p, 1, p, 1, 1, 8, 8, 1, 1, 64, 1.0, 0, 1, 0, None, 0, 0, None, None]
+    for at, v in ((0, 2), (1, None), (13, p + 8), (16, None), (17, None), (20, 4), (27, None), (38, 60), (41, 2), (41, 0), (45, -1), (45, 5), (2, 1 << 40), (5, 1 << 30)):
         assert lib.crog_packed_attn_bwd(*args[:at], v, *args[at + 1:]) == -1, at
     r = [1, p, 64, 64, p, 64, 64, p, 64, 64, p, 64, 64, p, 1, 4, p, p, 8, 1, 1, 64, 32, 1, 0, 0, None]
     for at, v in ((0, 2), (1, None), (13, None), (14, 0), (15, 2), (16, None), (18, -1), (22, 33), (22, 0), (23, 0)):
