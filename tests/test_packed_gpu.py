@@ -104,6 +104,9 @@ CASES = [
     ([300], [700], 2, 2, 120, True),
     ([676, 676], None, 2, 1, 64, False),
     ([1500, 37], None, 1, 8, 128, True),
+    ([400, 0, 5, 900], [400, 300, 5, 901], 3, 2, 32, False),      # dK / dV in shares: over a sequence without queries, from head to head
+    ([700, 260], [130, 500], 5, 1, 96, True),
+    ([640] * 34, None, 5, 1, 64, False),                          # ... more tiles than the device holds: several tiles in a share
 ]
 
 
