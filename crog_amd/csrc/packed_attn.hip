@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
     __syncthreads();
   }
   if (r >= rows) return;
-  if (h == 0 && blockIdx.y == 0) a.D[at] = Dr;
+  if (h == 0 && blockIdx.y == 0) a.D[at] = -Dr;      // (dK / dV begins its product with it)
   if (a.part_o) {
     store_row<float, DC>(a.part_o + ((long)blockIdx.y * a.kv_heads * a.group * a.rows_q + at) * dim, dq, h, dim, a.scale);
     return;
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(NT) packed_dq_sum_kernel(const PackedArgs a, i
 // inside: every key tile of a sequence starts with the same step.
 // The steps of all tiles lie one behind the other on one axis, each tile's with OPERANDS units more for its operands and results, and every block takes an
 // equal share of that axis (share > 0): causal or ragged tiles have anything between one step and thousands, and in pieces of equal length left CUs
-// idle for a quarter of the time (six causal sequences of up to 5000 rows, 16 / 4 heads of 128: 796 + 16 us to meet, in shares 638 + 26, 0.98
+// idle for a quarter of the time (six causal sequences of up to 5000 rows, 16 / 4 heads of 128: 796 + 16 us to meet, in shares 632 + 26, 0.99
 // PFLOP/s; where every block has as many steps in any case 1.1 PFLOP/s).  A tile that lies in several shares leaves a float sum in each, two places a block, which meet in
 // packed_meet_kernel in order.  share 0: a block a tile.
 // =====================================================================================================================
@@ -702,7 +702,8 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? DC <= 32 ? 4 : DC <= 64 ?
     for (int c = 0; c < L::NC; c++)
 #pragma unroll
       for (int i = 0; i < 16; i++) dk[c][i] = dv[c][i] = 0.f;
-    const float c2 = a.scale * LOG2E;
+    const float c2 = fabsf(a.scale) * LOG2E < 1e-30f ? 1e-30f : a.scale * LOG2E;      // (0 times a masked score's infinity would be NaN)
+    const float masked = c2 > 0.f ? -INFINITY : INFINITY;
     F fq, fg;
     fq.init(wave, lane, a.ldq);
     fg.init(wave, lane, a.lddo);
@@ -761,26 +762,29 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? DC <= 32 ? 4 : DC <= 64 ?
       opaque(at_c);
       f32x16 s, dp;
 #pragma unroll
-      for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
+      for (int g = 0; g < 4; g++) {
+        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&sS[buf][wave][1][8 * g + 4 * h]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          s[4 * g + j] = 0.f;
+          dp[4 * g + j] = d4[j];      // (-D: the product adds dO . v)
+        }
+      }
       __builtin_amdgcn_s_setprio(1);      // (products first, where the waves of a SIMD compete: 32 sequences of 676 tokens, a training pass 246 -> 221 us)
       mma_rows<T, DP, DC>(s, sQ[0], at_r, 0, kf);
       mma_rows<T, DP, DC>(dp, sG[0], at_r, 0, vf);
       __builtin_amdgcn_s_setprio(0);
       if (r0 < wall)
 #pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = r0 + acc_row(i, h) >= qmin ? s[i] * c2 : -INFINITY;
-      else
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] *= c2;
+        for (int i = 0; i < 16; i++) s[i] = r0 + acc_row(i, h) >= qmin ? s[i] : masked;
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         const f32x4 l4 = *reinterpret_cast<const f32x4*>(&sS[buf][wave][0][8 * g + 4 * h]);
-        const f32x4 d4 = *reinterpret_cast<const f32x4*>(&sS[buf][wave][1][8 * g + 4 * h]);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int i = 4 * g + j;
-          s[i] = ex2(s[i] - l4[j]);
-          dp[i] = s[i] * (dp[i] - d4[j]);      // (the scale follows at the end)
+          s[i] = ex2(s[i] * c2 - l4[j]);
+          dp[i] *= s[i];      // (the scale follows at the end)
         }
       }
       __builtin_amdgcn_s_setprio(1);

@@ -616,7 +616,7 @@ int crog_preprocess_u8(const uint8_t* img, const uint8_t* masks, int B, int H, i
  * j <= i + Lk - Lq (the ends aligned; a query that sees none gives zeros).  tiles: device int32 pairs (sequence, tile): blocks of 128 of the
  * sequence's Lq * group rows (forward, dQ: row_tiles) or of 128 keys (key_tiles), each exactly once, in the order in which they should start.
  * lse (may be NULL in the forward) and D: [kv_heads * group][rows_q] floats: the forward's base-2 log-sum-exp (+inf for a row without a key) for
- * the backward, and scratch of the backward (rowsum(dO * O)).
+ * the backward, and scratch of the backward (-rowsum(dO * O)).
  * splits > 1: the keys of a row are walked in `splits` pieces of split_keys (a multiple of 64; the last takes what is left) that meet in a second
  * launch; partial: splits * kv_heads * rows_q * group * (head_dim + 2) floats.
  * share > 0: a key tile's units - two, and one for each step of 32 queries (of a grid from the sequence's first) of one head that see it - lie
