@@ -148,6 +148,14 @@ __device__ inline void mma_cols(f32x16* out, const T* tile, int at, int tile_row
   }
 }
 
+// p becomes what the rounding of mma_cols leaves of it.  With few keys or few rows these roundings do not average out (two keys: dQ off by twice its
+// own rounding), so there, where a pass is launches and latency in any case, the rest goes through the matrix unit too.
+constexpr int FEW = 128;
+__device__ inline void leave_rest(f32x16& p) {
+#pragma unroll
+  for (int i = 0; i < 16; i++) p[i] -= (float)(bf16)p[i];
+}
+
 // the transposed operands of 16 tile rows from tile_row on, for all column blocks
 template <typename T, int DP, int DC>
 __device__ inline void load_cols(bf16x8* v, const T* tile, int at, int tile_row) {
@@ -233,7 +241,11 @@ template <typename T, int DP, int R> struct Fetch {
 };
 
 // =====================================================================================================================
-// forward.  grid (kv_heads * tiles, key splits); a block owns 128 rows of one sequence and key head, keys stream through LDS.
+// forward.  grid (kv_heads * tiles, key splits); a block owns 128 rows of one sequence and key head, keys stream through LDS in two buffers of 64.
+// Bound: at 128 columns the matrix units (one causal sequence of 16384 rows, 16 / 2 heads: 1045 us, 1.05 PFLOP/s; a large library product reaches 1.24
+// here), at 64 the vector work of the softmax beside them (a maximum, a fused step, an exponential, a sum and a conversion an element: 32 sequences of
+// 676 tokens, 8 heads: 50 us, 0.6 PFLOP/s), for single tokens memory (16 sequences of 200 to 8192 keys, 32 / 8 heads of 128: 71 + 5 us, 4.0 TB/s).  64
+// rows a wave instead of 32, one wave a SIMD: 1370 us for the long sequence.
 // =====================================================================================================================
 template <typename T, int DP, int DC, int NB>
 __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
@@ -350,17 +362,6 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
 #pragma unroll
           for (int c = 0; c < L::NC; c++) o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[g & 1][c], pb[g & 1], o[c], 0, 0, 0);
           if (g + 1 < G) probs(g + 1);
-#ifdef SGB
-          if (g + 1 < G) {
-          __builtin_amdgcn_sched_group_barrier(0x100, 2 * L::NC, 0);
-#pragma unroll
-          for (int c = 0; c < L::NC; c++) {
-            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x2, 20 / L::NC, 0);
-            __builtin_amdgcn_sched_group_barrier(0x400, 8 / L::NC, 0);
-          }
-          }
-#endif
         }
       } else {
 #pragma unroll
@@ -460,10 +461,11 @@ void launch_combine(const PackedArgs& a, int splits, int64_t total, hipStream_t 
 }
 
 // =====================================================================================================================
-// backward 1: D and dQ, blocked as the forward, its few rows over long keys cut in the same way (the float sums meet in packed_dq_sum_kernel).
+// backward 1: D and dQ, blocked as the forward, its few rows over long keys cut in the same way (the float sums meet in packed_dq_sum_kernel).  Three
+// products a tile: 1.1 PFLOP/s at 128 columns (four sequences of 4096 rows, 16 / 4 heads: 730 us), 0.66 at 64 (32 of 676 tokens, 8 heads: 68 us).
 // =====================================================================================================================
 template <typename T, int DP, int DC, int NB>
-__global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(NT, sizeof(T) == 2 && DC <= 32 ? 4 : 2) packed_bwd_dq_kernel(const PackedArgs a) {
   using L = Tile<T, DP, DC>;
   constexpr int KT = 32 * NB;
   __shared__ __attribute__((aligned(16))) T sK[2][KT * DP];
@@ -573,6 +575,10 @@ __global__ void __launch_bounds__(NT, 2) packed_bwd_dq_kernel(const PackedArgs a
         __builtin_amdgcn_s_setprio(1);
         mma_cols<T, DP, DC>(dq, sK[0], at_c, n * 32, s);
         __builtin_amdgcn_s_setprio(0);
+        if (sizeof(T) == 2 && min(rows, lim_hi) <= FEW) {
+          leave_rest(s);
+          mma_cols<T, DP, DC>(dq, sK[0], at_c, n * 32, s);
+        }
       }
     }
     wait_vmcnt<0>();
@@ -788,8 +794,14 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 ? DC <= 32 ? 4 : DC <= 64 ?
         }
       }
       __builtin_amdgcn_s_setprio(1);
-      mma_cols<T, DP, DC>(dv, sG[0], at_c, 0, s);
-      mma_cols<T, DP, DC>(dk, sQ[0], at_c, 0, dp);
+#pragma unroll 1
+      for (int again = sizeof(T) == 2 && e.lq <= FEW;; again--) {
+        mma_cols<T, DP, DC>(dv, sG[0], at_c, 0, s);
+        mma_cols<T, DP, DC>(dk, sQ[0], at_c, 0, dp);
+        if (!again) break;
+        leave_rest(s);
+        leave_rest(dp);
+      }
       __builtin_amdgcn_s_setprio(0);
     }
     if (key < e.lk && slot >= 0) {

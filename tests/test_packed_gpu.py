@@ -29,8 +29,9 @@ def within(got, want, bound, what):
 
 
 # ---- attention ------------------------------------------------------------------------------------------------------------------------------
-def attention_reference(q, k, v, do, lq, lk, causal, scale):
-    """float64 values and the bounds of the float32 / bf16 computation, sequence by sequence and head by head."""
+def attention_reference(q, k, v, do, lq, lk, causal, scale, few=False):
+    """float64 values and the bounds of the float32 / bf16 computation, sequence by sequence and head by head.  few: those of a backward pass of at
+    most 64 queries and keys a sequence, where the rest of each rounded operand follows it and D does not come from the stored o."""
     T = q.dtype
     h = H[T]
     hp = h if T == torch.bfloat16 else 0.0      # the rounding of the matrix unit's operand
@@ -62,14 +63,16 @@ def attention_reference(q, k, v, do, lq, lk, causal, scale):
             eo = (hp + ep + U * (m + 4)) * pv
             out["o"][a, hd] = o
             err["o"][a, hd] = h * o.abs() + eo * (1 + h)
+            hb = hp * 2.0 ** -8 if few else hp      # (the rest, at most half a step, is rounded by half a step of its own)
             out["dv"][b, e] += p.T @ gg
-            err["dv"][b, e] += (hp + U * (n * g + 4)) * (p.T @ gg.abs()) + (p * ep).T @ gg.abs()
+            err["dv"][b, e] += (hb + U * (n * g + 4)) * (p.T @ gg.abs()) + (p * ep).T @ gg.abs()
             dp = gg @ vv.T
             dd = (gg * o).sum(1, keepdim=True)
             ds = p * (dp - dd) * scale
             # D from the stored o (or, one key tile, from the probabilities: smaller)
-            edd = (gg.abs() * (h * o.abs() + eo * (1 + h))).sum(1, keepdim=True) + U * (D + m) * ((gg.abs() * o.abs()).sum(1, keepdim=True) + (p * dp.abs()).sum(1, keepdim=True))
-            eds = abs(scale) * p * (edd + U * (D + 4) * (gg.abs() @ vv.abs().T)) + ds.abs() * (hp + ep + 4 * U)
+            stored = ep * pv if few else h * o.abs() + eo * (1 + h)
+            edd = (gg.abs() * stored).sum(1, keepdim=True) + U * (D + m) * ((gg.abs() * o.abs()).sum(1, keepdim=True) + (p * dp.abs()).sum(1, keepdim=True))
+            eds = abs(scale) * p * (edd + U * (D + 4) * (gg.abs() @ vv.abs().T)) + ds.abs() * (hb + ep + 4 * U)
             out["dq"][a, hd] = ds @ kk
             err["dq"][a, hd] = h * out["dq"][a, hd].abs() + (eds @ kk.abs()) * (1 + h) + U * m * (ds.abs() @ kk.abs())
             out["dk"][b, e] += ds.T @ qq
@@ -128,6 +131,20 @@ def test_attention_matches_the_formula(case, dtype):
     from crog_amd import functional as Fn
     with torch.no_grad():
         assert torch.equal(Fn.packed_attention(q, k, v, rows), got["o"])
+
+
+@pytest.mark.parametrize("lq,lk,kv,group,dim,causal", [([2] * 30, None, 1, 1, 128, True), ([1, 2, 17, 64], [45, 2, 30, 64], 2, 2, 80, False),
+                                                       ([64, 5, 33], None, 3, 1, 32, True)])
+def test_attention_gradients_of_few_rows_are_rounded_once(lq, lk, kv, group, dim, causal):
+    from crog_amd.packed import PackedRows
+    rows = PackedRows(lq, lk, group=group, causal=causal)
+    lk = lk or lq
+    q, do = (dev(sum(lq), kv * group, dim, dtype=torch.bfloat16, seed=i) for i in (1, 2))
+    k, v = (dev(sum(lk), kv, dim, dtype=torch.bfloat16, seed=i) for i in (3, 4))
+    got = run_attention(q, k, v, do, rows)
+    want, bound = attention_reference(q, k, v, do, lq, lk, causal, dim ** -0.5, few=True)
+    for n in ("dq", "dk", "dv"):
+        within(got[n], want[n], bound[n], n)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
