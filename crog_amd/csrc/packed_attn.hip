@@ -525,8 +525,35 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 && DC <= 32 ? 4 : 2) packed
     fk.get(lds_k, kg, e.lk - kbeg, dim);
     fv.get(lds_v, vg, e.lk - kbeg, dim);
   }
+  const auto probs = [&](int kb, int at_r, int n, f32x16& s, f32x16& dp) {      // P and dP of 32 keys
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
+    __builtin_amdgcn_s_setprio(1);
+    mma_rows<T, DP, DC>(s, sK[0], at_r, n * 32, qf);
+    mma_rows<T, DP, DC>(dp, sV[0], at_r, n * 32, gf);
+    __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = s[i] * c2 - lse;
+    if (kb + KT > lim_lo)
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[i] = kb + n * 32 + acc_row(i, h) < lim ? s[i] : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = ex2(s[i]);
+  };
   wait_vmcnt<0>();
   __syncthreads();
+  if (kbeg == 0 && lim_lo <= KT && lim_hi > 0) {
+    float d = 0.f;
+#pragma unroll 1
+    for (int n = 0; n < NB; n++) {
+      f32x16 s, dp;
+      probs(0, rows_at, n, s, dp);
+#pragma unroll
+      for (int i = 0; i < 16; i++) d += s[i] * dp[i];
+    }
+    d = xor32_sum(d);
+    Dr = lim <= KT ? d : Dr;
+  }
   int buf = 0;
   for (int kb = kbeg; kb < kend; kb += KT, buf ^= 1) {
     const bool more = kb + KT < kend;
@@ -540,45 +567,20 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 2 && DC <= 32 ? 4 : 2) packed
       int at_r = rows_at + buf * KT * L::RB, at_c = cols_at + buf * KT * L::RB;
       opaque(at_r);
       opaque(at_c);
-      const bool whole = kb + KT <= lim_lo;
-      const auto probs = [&](int n, f32x16& s, f32x16& dp) {      // P and dP of 32 keys
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.f;
-        __builtin_amdgcn_s_setprio(1);
-        mma_rows<T, DP, DC>(s, sK[0], at_r, n * 32, qf);
-        mma_rows<T, DP, DC>(dp, sV[0], at_r, n * 32, gf);
-        __builtin_amdgcn_s_setprio(0);
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = s[i] * c2 - lse;
-        if (!whole)
-#pragma unroll
-          for (int i = 0; i < 16; i++) s[i] = kb + n * 32 + acc_row(i, h) < lim ? s[i] : -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[i] = ex2(s[i]);
-      };
       f32x16 s, dp;
-      if (kb == 0 && lim_lo <= KT) {
-        float d = 0.f;
-        for (int n = 0; n < NB; n++) {
-          probs(n, s, dp);
-#pragma unroll
-          for (int i = 0; i < 16; i++) d += s[i] * dp[i];
-        }
-        d = xor32_sum(d);
-        Dr = lim <= KT ? d : Dr;
-      }
 #pragma unroll
       for (int n = 0; n < NB; n++) {
-        probs(n, s, dp);
+        probs(kb, at_r, n, s, dp);
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = s[i] * (dp[i] - Dr);      // (the scale follows at the end)
         __builtin_amdgcn_s_setprio(1);
-        mma_cols<T, DP, DC>(dq, sK[0], at_c, n * 32, s);
-        __builtin_amdgcn_s_setprio(0);
-        if (sizeof(T) == 2 && min(rows, lim_hi) <= FEW) {
-          leave_rest(s);
+#pragma unroll 1
+        for (int again = sizeof(T) == 2 && min(rows, lim_hi) <= FEW;; again--) {
           mma_cols<T, DP, DC>(dq, sK[0], at_c, n * 32, s);
+          if (!again) break;
+          leave_rest(s);
         }
+        __builtin_amdgcn_s_setprio(0);
       }
     }
     wait_vmcnt<0>();
