@@ -529,6 +529,45 @@ def test_gated_norm_of_no_rows():
     assert u.shape == h.shape == dx.shape == dy.shape == (0, 64) and (st.G == 0).all()
 
 
+def test_rotary_and_gated_norm_captured_and_replayed():
+    """Captured forward and backward passes, replayed on new inputs beside eager work: outputs, gradients and the weights' gradients, added on."""
+    from crog_amd import functional as Fn
+    from crog_amd.packed import RotaryAxes
+    T, C = 300, 192
+    axes = RotaryAxes((8, 24))
+    _, st, r = store_of(C, ["gate", "post_w", "pre_w", "pre_b"], 2)
+    x, y, gu, gh = (dev(T, C, dtype=torch.bfloat16, seed=i) for i in (1, 2, 3, 4))
+    pos = torch.arange(2 * T, device="cuda").view(T, 2)
+    x.requires_grad_(), y.requires_grad_()
+
+    def step():
+        q, _ = Fn.rotary(y.view(T, 3, 64), None, pos, axes)
+        u, h = Fn.gated_norm(x, q.reshape(T, C), post=(r["post_w"], None), gate=r["gate"], pre=(r["pre_w"], r["pre_b"]))
+        return (u, h, *torch.autograd.grad((u, h), (x, y), (gu, gh)))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = step()
+    for turn in range(4):
+        with torch.no_grad():
+            for i, t in enumerate((x, y, gu, gh)):
+                t.copy_(dev(T, C, dtype=torch.bfloat16, seed=10 * turn + i))
+            pos.add_(turn)
+        st.zero_grad()
+        want = step()
+        once = st.G.clone()
+        st.zero_grad()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want)) and torch.equal(st.G, once), turn
+        g.replay()
+        assert torch.equal(st.G, once + once), turn
+
+
 def test_one_block_on_packed_rows_trains():
     """The operators as a block uses them - norm, projections, rotary, packed attention, gated residual - forward and backward, against the same
     block in float64: every gradient within a bf16 step's worth of the largest of its tensor, in float32 within 2^-14."""
