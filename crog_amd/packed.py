@@ -38,7 +38,7 @@ def _lengths(name: str, lengths: Sequence[int]) -> np.ndarray:
             raise TypeError(f"PackedRows: {name} are host numbers (a list, or a CPU tensor): the launch grid depends on them")
         lengths = lengths.tolist()
     out = [operator.index(n) for n in lengths]
-    if any(n < 0 for n in out):
+    if min(out, default=0) < 0:
         raise ValueError(f"PackedRows: {name} must not be negative")
     if sum(out) > 0x7fffff00:
         raise ValueError(f"PackedRows: {sum(out)} rows are too many")
@@ -46,14 +46,15 @@ def _lengths(name: str, lengths: Sequence[int]) -> np.ndarray:
 
 
 def _tiles(rows: np.ndarray, size: int, cost, together: bool = False):
-    """[(sequence, tile)] of all tiles of `size` rows and their costs, the costliest first (a late long one would leave the device waiting for a
+    """Sequences, numbers and costs of all tiles of `size` rows, the costliest first (a late long one would leave the device waiting for a
     single block); together: a sequence's tiles one behind the other, the sequence with the costliest first."""
     n = (rows + size - 1) // size
-    seq = np.repeat(np.arange(len(rows)), n)
-    tile = np.arange(len(seq)) - np.repeat(np.cumsum(n) - n, n)
+    ends = n.cumsum()
+    seq = np.arange(len(rows)).repeat(n)
+    tile = np.arange(len(seq)) - (ends - n).repeat(n)
     c = cost(seq, tile)
-    order = np.argsort(-(cost(seq, 0) if together else c), kind="stable")
-    return np.stack([seq[order], tile[order]], 1), c[order]
+    order = (-(cost(seq, 0) if together else c)).argsort(kind="stable")
+    return seq[order], tile[order], c[order]
 
 
 class PackedRows:
@@ -81,28 +82,35 @@ class PackedRows:
         g, c = self.group, self.causal
 
         def row_cost(s, t):      # keys of the tile's last row
+            if not c:
+                return lk[s]
             last = np.minimum(t * TILE + TILE - 1, lq[s] * g - 1) // g
-            return np.clip(last + 1 + lk[s] - lq[s], 0, lk[s]) if c else lk[s]
+            return np.minimum(np.maximum(last + 1 + lk[s] - lq[s], 0), lk[s])
 
-        def key_cost(s, t):      # steps of the tile: 32 queries of one head each, from the block that first sees its first key to the last
-            first = np.clip(t * KEY_TILE - (lk[s] - lq[s]), 0, lq[s]) if c else 0
-            return ((lq[s] + STEP - 1) // STEP - first // STEP) * g
+        def key_cost(s, t):      # steps of the tile (32 queries of one head each, from the block that first sees its first key to the last), and its operands
+            lqs = lq[s]
+            steps = (lqs + STEP - 1) // STEP
+            if c:
+                steps = steps - np.minimum(np.maximum(t * KEY_TILE - (lk[s] - lqs), 0), lqs) // STEP
+            return steps * g + OPERANDS
 
-        (rt, _), (kt, kc) = _tiles(lq * g, TILE, row_cost), _tiles(lk, KEY_TILE, key_cost, together=True)
-        kc = kc + OPERANDS
-        self.key_units, self.key_most = int(kc.sum()), int(kc.max()) if len(kc) else 0
-        self.n_row_tiles, self.n_key_tiles = len(rt), len(kt)
-        zero = np.zeros(1, dtype=np.int64)
-        parts = [np.concatenate([zero, np.cumsum(lq)]), np.concatenate([zero, np.cumsum(lk)]), rt.reshape(-1), kt.reshape(-1),
-                 np.concatenate([zero, np.cumsum(kc)]) if self.key_units < 1 << 31 else zero]
-        table = torch.from_numpy(np.concatenate(parts).astype(np.int32))
-        self._table = table.to(device)      # one copy; the tables lie in it one behind the other
+        rs, rt, _ = _tiles(lq * g, TILE, row_cost)
+        ks, kt, kc = _tiles(lk, KEY_TILE, key_cost, together=True)
+        self.n_row_tiles, self.n_key_tiles = nr, nk = len(rt), len(kt)
+        units = kc.cumsum()
+        self.key_units, self.key_most = (int(units[-1]), int(kc.max())) if nk else (0, 0)
+        # the tables one behind the other, in one copy: the sequences' ends on both sides, (sequence, tile) of the row tiles and the key tiles, the
+        # units before each key tile and of all
+        n = self.seqs + 1
+        at = np.array([0, n, 2 * n, 2 * (n + nr), 2 * (n + nr + nk)])
+        table = np.zeros(at[-1] + nk + 1, dtype=np.int32)
+        table[1:n], table[n + 1:2 * n] = lq.cumsum(), lk.cumsum()
+        table[at[2]:at[3]:2], table[at[2] + 1:at[3]:2], table[at[3]:at[4]:2], table[at[3] + 1:at[4]:2] = rs, rt, ks, kt
+        if self.key_units < 1 << 31:
+            table[at[4] + 1:] = units
+        self._table = torch.from_numpy(table).to(device)
         self.device, self.made_on = self._table.device, _stream_of(self._table)
-        at, addr = 0, []
-        for p in parts:
-            addr.append(self._table.data_ptr() + 4 * at)
-            at += len(p)
-        self.cu_q_ptr, self.cu_k_ptr, self.row_tiles_ptr, self.key_tiles_ptr, self.key_units_ptr = addr
+        self.cu_q_ptr, self.cu_k_ptr, self.row_tiles_ptr, self.key_tiles_ptr, self.key_units_ptr = (self._table.data_ptr() + 4 * at).tolist()
 
     def splits(self, kv_heads: int, size: int):
         """(pieces, keys of a piece) of the forward and dQ passes' key axis; size: bytes of an element.  A single query over 8192 keys of 8 heads
