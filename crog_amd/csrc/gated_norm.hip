@@ -9,8 +9,8 @@
 // so four column sums (dU Y, dU, dh U, dh) give all five.
 //
 // Bound: memory.  Forward reads x, y and writes u, h (the next row is fetched during this one: 77 -> 46 us at 32768 x 1024 bf16, 268 MB, 5.8 TB/s);
-// backward reads x, y, du, dh and writes dx, dy (403 MB, 90 us, 4.5 TB/s).  The weights stay in registers while a group of TPR threads walks over
-// rows.  A thread holds at most 16 columns (four sums and four weights each are 128 registers): a row takes 16, 64, 256 or 512 threads.  Column sums: registers, then the block's groups through LDS, then one slab row per block, added up in block order by a
+// backward reads x, y, du, dh and writes dx, dy (403 MB, 91 us, 4.4 TB/s).  The weights stay in registers or LDS while a group of TPR threads walks
+// over rows.  A thread holds at most 16 columns (four sums and four weights each are 128 registers): a row takes 16, 64, 256 or 512 threads.  Column sums: registers, then the block's groups through LDS, then one slab row per block, added up in block order by a
 // second launch - no atomics, the same bits every time.
 #include "common.h"
 
@@ -197,48 +197,85 @@ __device__ inline void normalise_back(float (&d)[N], const float (&n)[N], int t,
 }
 
 template <typename T, int TPR, int NV, bool WHOLE>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_bwd_kernel(const GnArgs a) {
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256, 2) gated_norm_bwd_kernel(const GnArgs a) {
   using S = Threads<T, TPR, NV, WHOLE>;
   __shared__ float slots[S::THREADS / 32];
   Meet red{slots, 0};
   __shared__ float part[S::GROUPS > 1 ? S::THREADS : 1];
   const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
-  float gate[S::N], w1[S::N], b1[S::N], w2[S::N];
-  load_weights<S>(gate, a.gate, 1.f, t, a.cols);
-  load_weights<S>(w1, a.post_w, 1.f, t, a.cols);
-  load_weights<S>(b1, a.post_b, 0.f, t, a.cols);
-  load_weights<S>(w2, a.pre_w, 1.f, t, a.cols);
+  // The weights (gate, post_w, post_b, pre_w) in registers, where they leave no room for the next row beside the four sums; or in LDS, with the next
+  // row on its way: rows read element by element (16000 x 1021 bf16: 154 -> 116 us) and of at most 256 columns (40000 x 256: 49 -> 36), but longer
+  // ones lose more to the reads than they gain (32768 x 1024: 91 -> 128).
+  constexpr bool AHEAD = TPR == 16 || (!WHOLE && TPR <= 256);
+  __shared__ __attribute__((aligned(16))) float wts[4][AHEAD ? TPR * S::N : 1];
+  float wreg[4][AHEAD ? 1 : S::N];
+  const float* const from[4] = {a.gate, a.post_w, a.post_b, a.pre_w};
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const float otherwise = k == 2 ? 0.f : 1.f;
+    if constexpr (AHEAD) {
+      for (int c = threadIdx.x; c < TPR * S::N; c += S::THREADS) wts[k][c] = c < a.cols ? (from[k] ? from[k][c] : otherwise) : 0.f;
+    } else {
+      load_weights<S>(wreg[k], from[k], otherwise, t, a.cols);
+    }
+  }
+  if constexpr (AHEAD) __syncthreads();
   float sum[4][S::N];      // dU Y, dU, dh U, dh
 #pragma unroll
   for (int k = 0; k < 4; k++)
 #pragma unroll
     for (int i = 0; i < S::N; i++) sum[k][i] = 0.f;
-  for (int base = blockIdx.x * S::GROUPS; base < a.rows; base += gridDim.x * S::GROUPS) {
-    const int row = base + grp, rc = min(row, a.rows - 1);
-    const bool live = row < a.rows, both = a.has_pre && a.dh;
-    const f32x4 st = *reinterpret_cast<const f32x4*>(a.stats + 4 * (long)rc);
-    const Row<T, NV> ry = fetch<T, TPR, NV, WHOLE>(a.y, a.ldy, rc, t, a.cols);
-    Row<T, NV> rx{}, rh{}, ru{};
+  struct Next {
+    f32x4 st;
+    Row<T, NV> x, y, du, dh;
+  };
+  const bool both = a.has_pre && a.dh;
+  const auto request = [&](int row) {
+    Next next{};
+    const int rc = min(row, a.rows - 1);
+    next.st = *reinterpret_cast<const f32x4*>(a.stats + 4 * (long)rc);
+    next.y = fetch<T, TPR, NV, WHOLE>(a.y, a.ldy, rc, t, a.cols);
     if (both) {
-      rx = fetch<T, TPR, NV, WHOLE>(a.x, a.ldx, rc, t, a.cols);
-      rh = fetch<T, TPR, NV, WHOLE>(a.dh, a.lddh, rc, t, a.cols);
+      next.x = fetch<T, TPR, NV, WHOLE>(a.x, a.ldx, rc, t, a.cols);
+      next.dh = fetch<T, TPR, NV, WHOLE>(a.dh, a.lddh, rc, t, a.cols);
     }
-    if (a.du) ru = fetch<T, TPR, NV, WHOLE>(a.du, a.lddu, rc, t, a.cols);
+    if (a.du) next.du = fetch<T, TPR, NV, WHOLE>(a.du, a.lddu, rc, t, a.cols);
+    return next;
+  };
+  const int step = gridDim.x * S::GROUPS;
+  Next next;
+  if constexpr (AHEAD) next = request(blockIdx.x * S::GROUPS + grp);
+  for (int base = blockIdx.x * S::GROUPS; base < a.rows; base += step) {
+    const int row = base + grp;
+    const bool live = row < a.rows;
+    int lane = t;
+    if constexpr (AHEAD) asm volatile("" : "+v"(lane));      // (or the weights in LDS would be read once, into registers)
+    const auto w = [&](int k, int i) {
+      if constexpr (AHEAD) return wts[k][S::col(lane, i)];
+      else return wreg[k][i];
+    };
+    Next now;
+    if constexpr (AHEAD) now = next;
+    else now = request(row);
+    const f32x4 st = now.st;
     float y[S::N], d[S::N];      // Y (y itself without a post norm), dU
-    widen(y, ry);
+    widen(y, now.y);
+    if constexpr (AHEAD) {
+      if (base + step < a.rows) next = request(row + step);
+    }
     if (a.has_post)
 #pragma unroll
       for (int i = 0; i < S::N; i++) y[i] = S::has(t, i, a.cols) ? (y[i] - st[0]) * st[1] : 0.f;
     if (both) {
       float u[S::N], g[S::N];
-      widen(u, rx);
-      widen(g, rh);
+      widen(u, now.x);
+      widen(g, now.dh);
 #pragma unroll
       for (int i = 0; i < S::N; i++) {
-        const float z = a.has_post ? y[i] * w1[i] + b1[i] : y[i];
-        u[i] = S::has(t, i, a.cols) ? (a.alpha * u[i] + gate[i] * z - st[2]) * st[3] : 0.f;
+        const float z = a.has_post ? y[i] * w(1, i) + w(2, i) : y[i];
+        u[i] = S::has(t, i, a.cols) ? (a.alpha * u[i] + w(0, i) * z - st[2]) * st[3] : 0.f;
         if (live) { sum[2][i] += g[i] * u[i]; sum[3][i] += g[i]; }
-        d[i] = g[i] * w2[i];
+        d[i] = g[i] * w(3, i);
       }
       normalise_back<TPR, S>(d, u, t, a.cols, a.rms, st[3], red);
     } else {
@@ -247,7 +284,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_bwd_kernel(c
     }
     if (a.du) {
       float g[S::N];
-      widen(g, ru);
+      widen(g, now.du);
 #pragma unroll
       for (int i = 0; i < S::N; i++) d[i] += g[i];
     }
@@ -256,7 +293,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) gated_norm_bwd_kernel(c
     for (int i = 0; i < S::N; i++) {
       if (live) { sum[0][i] += d[i] * y[i]; sum[1][i] += d[i]; }
       o[i] = a.alpha * d[i];
-      d[i] = a.has_post ? d[i] * gate[i] * w1[i] : d[i] * gate[i];
+      d[i] = a.has_post ? d[i] * w(0, i) * w(1, i) : d[i] * w(0, i);
     }
     if (live && a.dx) store_row<T, TPR, WHOLE>(a.dx, a.lddx, row, o, t, a.cols);
     if (a.has_post) normalise_back<TPR, S>(d, y, t, a.cols, a.rms, st[1], red);
