@@ -28,7 +28,8 @@ struct GnArgs {
 };
 
 // Rows whose length is a whole number of 16-byte vectors and whose tensors are 16-byte aligned (WHOLE) are read vector by vector, and a thread's
-// vector is there or it is not; other rows element by element.
+// vector is there or it is not; of other rows the whole vectors by unaligned accesses, which the memory path takes (16000 x 1021 bf16, forward: 80 us
+// element by element, 52 so), the end element by element.
 template <typename T, bool WHOLE>
 __device__ inline Vec16<T> load_vec(const T* row, int c0, int cols) {
   constexpr int V = Elem<T>::VEC;
@@ -37,6 +38,8 @@ __device__ inline Vec16<T> load_vec(const T* row, int c0, int cols) {
     f32x4 q = {0.f, 0.f, 0.f, 0.f};
     if (c0 < cols) q = *reinterpret_cast<const f32x4*>(row + c0);
     v = __builtin_bit_cast(Vec16<T>, q);
+  } else if (c0 + V <= cols) {
+    __builtin_memcpy(&v, row + c0, sizeof(v));
   } else {
 #pragma unroll
     for (int e = 0; e < V; e++)
@@ -52,6 +55,11 @@ __device__ inline void store_vec(T* row, const float* f, int c0, int cols) {
 #pragma unroll
     for (int e = 0; e < V; e++) v.v[e] = Elem<T>::from_f(f[e]);
     if (c0 < cols) stg16(row + c0, v);
+  } else if (c0 + V <= cols) {
+    Vec16<T> v;
+#pragma unroll
+    for (int e = 0; e < V; e++) v.v[e] = Elem<T>::from_f(f[e]);
+    __builtin_memcpy(row + c0, &v, sizeof(v));
   } else {
 #pragma unroll
     for (int e = 0; e < V; e++)
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, 2) gated_norm_bwd_kerne
   __shared__ float part[S::GROUPS > 1 ? S::THREADS : 1];
   const int t = threadIdx.x % TPR, grp = threadIdx.x / TPR;
   // The weights (gate, post_w, post_b, pre_w) in registers, where they leave no room for the next row beside the four sums; or in LDS, with the next
-  // row on its way: rows read element by element (16000 x 1021 bf16: 154 -> 116 us) and of at most 256 columns (40000 x 256: 49 -> 36), but longer
+  // row on its way: rows with an odd end (16000 x 1021 bf16: 116 us of 154 before) and of at most 256 columns (40000 x 256: 36 of 49), but longer
   // ones lose more to the reads than they gain (32768 x 1024: 91 -> 128).
   constexpr bool AHEAD = TPR == 16 || (!WHOLE && TPR <= 256);
   __shared__ __attribute__((aligned(16))) float wts[4][AHEAD ? TPR * S::N : 1];
