@@ -101,7 +101,7 @@ def _needs_rebuild(obj: str, deps):
 def build(verbose: bool = False, force: bool = False) -> str:
     """Compile every HIP source for gfx950 and link crog_amd/libcrog_hip.so (in-tree)."""
     os.makedirs(BUILD_DIR, exist_ok=True)
-    common = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_dma.h"), os.path.join(CSRC, "comm_dev.h"), HEADER,
+    common = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "gemm_dma.h"), os.path.join(CSRC, "comm_dev.h"), os.path.join(CSRC, "packed_share.h"), HEADER,
               os.path.abspath(__file__)]      # (this file holds the compile flags)
     hipcc = os.environ.get("HIPCC", "hipcc")
 

@@ -1,0 +1,114 @@
+"""What keeps the packed operators inside their memory and their promises, without a GPU: the shares of the dK / dV pass compiled for the host."""
+import os
+import random
+import subprocess
+
+import pytest
+
+from crog_amd import _lib
+from crog_amd.packed import KEY_TILE, PackedRows
+
+WALK = r'''
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+#include "packed_share.h"
+// the walk of packed_bwd_dkdv_kernel over the shares and of packed_meet_kernel over the tiles: prints what every block and tile does
+int main() {
+  int n, total, kv, share, blocks;
+  while (scanf("%d %d %d %d %d", &n, &total, &kv, &share, &blocks) == 5) {
+    std::vector<int> units(n + 1), steps(n);
+    for (int& u : units) if (scanf("%d", &u) != 1) return 1;
+    for (int& s : steps) if (scanf("%d", &s) != 1) return 1;
+    printf("case\n");
+    const int grid = (blocks + 7) / 8 * 8;
+    for (int b = 0; b < grid; b++) {
+      const Place p = place_of(units.data(), n, total, kv, share, b);
+      if (p.pos >= p.end) continue;
+      long pos = p.pos;
+      int kh = p.kh, ti = p.ti, rounds = 0;
+      while (pos < p.end) {
+        if (kh < 0 || kh >= kv || ti < 0 || ti >= n) { printf("outside\n"); return 0; }
+        const Segment s = segment_of(pos, p.end, b, (long)kh * units[n] + units[ti], units_of(units.data(), ti), steps[ti]);
+        printf("walk %d %d %d %d %d %d\n", b, kh, ti, s.first, s.last, s.slot);
+        if (s.next <= pos || ++rounds > share) { printf("endless\n"); return 0; }
+        pos = s.next;
+        if (++ti == n) { ti = 0; kh = kh + 1 < kv ? kh + 1 : kv - 1; }
+      }
+    }
+    for (int kh = 0; kh < kv; kh++)
+      for (int t = 0; t < n; t++) {
+        const Meeting m = meeting_of((long)kh * total + units[t], units_of(units.data(), t), share, blocks);
+        if (m.first < m.last) printf("meet %d %d %d %d\n", kh, t, m.first, m.last);
+      }
+  }
+}
+'''
+
+
+@pytest.fixture(scope="module")
+def walk(tmp_path_factory):
+    d = tmp_path_factory.mktemp("share")
+    (d / "walk.cpp").write_text(WALK)
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", "-I", _lib.CSRC, str(d / "walk.cpp"), "-o", str(d / "walk")])
+
+    def run(n, total, kv, share, blocks, units, steps):
+        text = " ".join(map(str, [n, total, kv, share, blocks, *units, *steps]))
+        out = subprocess.run([str(d / "walk")], input=text, capture_output=True, text=True, timeout=60)
+        assert out.returncode == 0, out.stderr
+        assert "outside" not in out.stdout and "endless" not in out.stdout
+        rows = [line.split() for line in out.stdout.splitlines()[1:]]
+        return [tuple(map(int, r[1:])) for r in rows if r[0] == "walk"], [tuple(map(int, r[1:])) for r in rows if r[0] == "meet"]
+    return run
+
+
+def plan(lq, lk, group, causal):
+    p = PackedRows(lq, lk, group=group, causal=causal, device="cpu")
+    t = p._table.numpy()
+    pairs = t[2 * (p.seqs + 1) + 2 * p.n_row_tiles:][:2 * p.n_key_tiles].reshape(-1, 2)
+    lk = lk or lq
+    first = [min(max(k * KEY_TILE - (lk[s] - lq[s]), 0), lq[s]) if causal else 0 for s, k in pairs.tolist()]
+    steps = [(-(-lq[s] // 32) - f // 32) * group for (s, _), f in zip(pairs.tolist(), first)]
+    return p, t[-p.n_key_tiles - 1:].tolist(), steps
+
+
+PLANS = [([5000, 300], None, 4, 4, True), ([4096], None, 8, 1, True), ([400, 0, 5, 900], [400, 300, 5, 901], 2, 3, False), ([3000], [100], 2, 1, True),
+         ([700, 260], [130, 500], 1, 5, True)]
+
+
+@pytest.mark.parametrize("lq,lk,group,kv,causal", PLANS)
+def test_shares_walk_every_step_once_and_meet_where_they_left_sums(walk, lq, lk, group, kv, causal):
+    p, units, steps = plan(lq, lk, group, causal)
+    for share in (1, 3, 8, 50, 1000):
+        blocks = -(-p.key_units * kv // share)
+        walks, meets = walk(p.n_key_tiles, p.key_units, kv, share, blocks, units, steps)
+        seen, slots = {}, {}
+        for b, kh, t, first, last, slot in walks:
+            seen.setdefault((kh, t), []).append((first, last))
+            if slot >= 0:
+                assert 0 <= slot < 2 * blocks and slot not in slots
+                slots[slot] = (kh, t)
+        assert set(seen) == {(kh, t) for kh in range(kv) for t in range(p.n_key_tiles)}
+        for (kh, t), parts in seen.items():
+            assert parts[0][0] == 0 and parts[-1][1] == steps[t] and all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
+        met = {2 * b + (b == first): (kh, t) for kh, t, first, last in meets for b in range(first, last + 1)}
+        assert met == slots
+
+
+@pytest.mark.parametrize("lq,lk,group,kv,causal", PLANS)
+def test_shares_stay_in_their_workspace_whatever_the_table_holds(walk, lq, lk, group, kv, causal):
+    """A table whose memory was given away (a plan dropped while a graph that was captured with it is still replayed): too many units, none at all,
+    anything."""
+    p, units, steps = plan(lq, lk, group, causal)
+    n, total = p.n_key_tiles, p.key_units
+    rng = random.Random(1)
+    wrong = [units[:-1] + [units[-1] + 1000 * kv], [0] * (n + 1), [u + 7 for u in units], units[::-1], [0x7fffffff] * (n + 1), [-0x80000000, 0x7fffffff] * n,
+             *[[rng.randrange(-(1 << 31), 1 << 31) for _ in range(n + 1)] for _ in range(5)], *[[rng.randrange(0, 2 * total) for _ in range(n + 1)] for _ in range(5)]]
+    for table in wrong:
+        for share in (3, 50, total):
+            blocks = -(-total * kv // share)
+            walks, meets = walk(n, total, kv, share, blocks, (table + table)[:n + 1], steps)
+            for b, kh, t, first, last, slot in walks:
+                assert -1 <= slot < 2 * blocks and 0 <= first <= last <= steps[t], (table, share)
+            for kh, t, first, last in meets:
+                assert 0 <= first and last < blocks
