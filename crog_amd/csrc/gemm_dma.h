@@ -20,6 +20,7 @@ constexpr unsigned DMA_OOB = 0x80000000u;
 #ifndef CROG_ASM_DMA
 #define CROG_ASM_DMA 1
 #endif
+// The text holds the wait state that the hardware wants between the write of M0 and a load that goes to LDS by it (the compiler's own such pairs have it).
 typedef int dma_i32x4 __attribute__((ext_vector_type(4)));
 __device__ __attribute__((always_inline)) inline void dma_piece(const void* base, int extent, char* dst, unsigned off) {
 #ifdef CROG_PROBE_NO_OOB      // probe build (LAB_NOTES section 10): no lane is ever out of range - border taps read the operand's first bytes (WRONG values, on purpose)
@@ -34,7 +35,7 @@ __device__ __attribute__((always_inline)) inline void dma_piece(const void* base
   r.z = __builtin_amdgcn_readfirstlane(extent);
   r.w = 0x00020000;
   const unsigned m0v = __builtin_amdgcn_readfirstlane((unsigned)(unsigned long)(lds_char*)dst);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0v), "v"(off), "s"(r) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0v), "v"(off), "s"(r) : "memory", "m0");
 #else
   typedef __attribute__((address_space(3))) void lds_void;
   __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, extent, 0x00020000);

@@ -48,7 +48,7 @@ __device__ inline Seq seq_of(const PackedArgs& a, int s) {
 }
 
 // ---- LDS tiles of rows of DP elements ----------------------------------------------------------------------------------------
-// gemm_dma.h's request, to an LDS byte address and with a scalar offset besides the lane's (both below 2^31: their sum is out of range exactly where
+// gemm_dma.h's request (its wait state after M0 too), to an LDS byte address and with a scalar offset besides the lane's (both below 2^31: their sum is out of range exactly where
 // the lane's is DMA_OOB)
 __device__ __attribute__((always_inline)) inline void dma_piece_at(const void* base, unsigned lds, unsigned off, unsigned soff) {
   const unsigned long long b = (unsigned long long)base;
@@ -57,7 +57,7 @@ __device__ __attribute__((always_inline)) inline void dma_piece_at(const void* b
   r.y = __builtin_amdgcn_readfirstlane((int)((unsigned)(b >> 32) & 0xffffu));
   r.z = 0x7fffffff;
   r.w = 0x00020000;
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(soff) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(off), "s"(r), "s"(soff) : "memory", "m0");
 }
 // the same with 4 bytes a lane
 __device__ __attribute__((always_inline)) inline void dma_word_at(const void* base, unsigned lds, unsigned off) {
@@ -67,7 +67,7 @@ __device__ __attribute__((always_inline)) inline void dma_word_at(const void* ba
   r.y = __builtin_amdgcn_readfirstlane((int)((unsigned)(b >> 32) & 0xffffu));
   r.z = 0x7fffffff;
   r.w = 0x00020000;
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(r) : "memory", "m0");
 }
 __device__ inline unsigned lds_of(const void* p) {      // the LDS byte address of a shared array
   typedef __attribute__((address_space(3))) const char lds_char;

@@ -1,6 +1,7 @@
 """What keeps the packed operators inside their memory and their promises, without a GPU: the shares of the dK / dV pass compiled for the host."""
 import os
 import random
+import re
 import subprocess
 
 import pytest
@@ -112,3 +113,50 @@ def test_shares_stay_in_their_workspace_whatever_the_table_holds(walk, lq, lk, g
                 assert -1 <= slot < 2 * blocks and 0 <= first <= last <= steps[t], (table, share)
             for kh, t, first, last in meets:
                 assert 0 <= first and last < blocks
+
+
+def test_requests_into_lds_hold_their_wait_states(tmp_path):
+    """A request into LDS as inline assembly: the hardware wants one wait state between the write of M0 and a load that goes to LDS by it, and five between a
+    vector instruction's write of a scalar register (readfirstlane, readlane) and a load that reads it.  The compiler puts both in front of its own
+    instructions, but not into a text of ours."""
+    found = 0
+    for name in sorted(os.listdir(_lib.CSRC)):
+        if not name.endswith((".hip", ".h")):
+            continue
+        for text in re.findall(r'asm volatile\("((?:[^"\\]|\\.)*)"', open(os.path.join(_lib.CSRC, name)).read()):
+            lines = text.replace("\\t", "").split("\\n")
+            for before, line in zip([""] + lines, lines):
+                if line.startswith("buffer_load") and line.endswith(" lds"):
+                    found += 1
+                    assert before.startswith("s_nop"), (name, text)
+    assert found >= 3
+
+    out = tmp_path / "packed_attn.s"
+    flags = [f for f in _lib.HIPCC_FLAGS if f != "-fPIC"]
+    subprocess.check_call(["hipcc"] + flags + ["-S", "--cuda-device-only", os.path.join(_lib.CSRC, "packed_attn.hip"), "-o", str(out)], stderr=subprocess.DEVNULL)
+    lines = [line.split(";")[0].strip() for line in out.read_text().splitlines()]
+    lines = [line for line in lines if line and line[0] not in ".#"]
+
+    def scalars(text):
+        got = set()
+        for lo, hi, one in re.findall(r"\bs\[(\d+):(\d+)\]|\bs(\d+)\b", text):
+            got |= set(range(int(lo), int(hi) + 1)) if lo else {int(one)}
+        return got
+    requests = 0
+    for i, line in enumerate(lines):
+        if not (line.startswith("buffer_load") and line.endswith(" lds")):
+            continue
+        requests += 1
+        need, waits, moved = scalars(line), 0, 0
+        for before in reversed(lines[max(i - 8, 0):i]):
+            if before.endswith(":"):
+                continue
+            if re.match(r"s_\w+ m0,", before):
+                moved = waits
+                assert moved >= 1, (i, before, line)
+            if before.startswith("v_") and waits < 5:
+                first = before.split(None, 1)[1].split(",")[0] if " " in before else ""
+                assert not scalars(first) & need, (i, before, line)
+            waits += int(before.split()[1]) + 1 if before.startswith("s_nop") else 1
+        assert moved
+    assert requests > 500
