@@ -1419,10 +1419,8 @@ class GatedNormFn(Function):
         slab = K.gated_norm_bwd(x, y, du, dh, weights, post is not None, pre is not None, rms, alpha, stats, dx, dy, bool(live))
         if live:
             M, C = stats.shape[0], x.shape[-1]
-            if RT._join_armed:      # this backward pass writes gradients on the weight-gradient stream: behind them, should a weight be shared
-                RT.on_wgrad_stream(lambda: K.gated_norm_sums(slab, M, C, weights, post is not None, grads), slab, tag="ln")
-            else:
-                K.gated_norm_sums(slab, M, C, weights, post is not None, grads)
+            # (in one order with whatever else adds onto a weight that is shared)
+            RT.add_gradients(lambda: K.gated_norm_sums(slab, M, C, weights, post is not None, grads), slab, joined=dx is not None or dy is not None, tag="ln")
             done_joint(live.values())
         return (dx, dy) + none
 
@@ -1432,7 +1430,8 @@ def gated_norm(x, y, *, post=None, gate: Optional[WRef] = None, pre=None, res_sc
     h = norm(u) with `pre`; -> (u, h), h None without `pre`.  post / pre: (weight WRef, bias WRef or None); gate: WRef of one factor per column
     (1 without it).  rms: root-mean-square norms (no biases) instead of LayerNorm.  x, y: row matrices [..., C] of one shape and dtype, C up to
     8192; the second norm reads the float32 sum, u and h are rounded once.  The weights' gradients are added into the flat store in a fixed
-    order (same bits every time).  One weight may stand in several places."""
+    order (same bits every time).  One weight may stand in several places, of one call or of several, on whatever streams; only under
+    DistributedDataParallel a parameter belongs to one call a pass (the first that has added onto it announces it to its bucket)."""
     K.dcode(x)
     if x.shape != y.shape or x.dtype != y.dtype or x.dim() < 1:
         raise ValueError(f"gated_norm: x and y must have one shape and dtype, got {tuple(x.shape)} {x.dtype} and {tuple(y.shape)} {y.dtype}")

@@ -99,6 +99,7 @@ class Runtime:
         self.aux_stream = None
         self._streams_ready = False
         self._join_armed = False
+        self._direct = None      # where add_gradients last added on a node's own stream: (its raw handle, the stream)
         # deterministic mode (set_deterministic below; CROG_DETERMINISTIC=1): every sum whose order would depend on atomics takes its
         # ordered form - same inputs, same bits, run after run, eager or replayed
         self.deterministic = False
@@ -329,9 +330,43 @@ class Runtime:
                 for d in done:
                     d()
 
+    def add_gradients(self, fn, *tensors, joined, tag=None):
+        """Run fn() (launches that add onto parameter gradients by a plain read, add and write) like on_wgrad_stream does, but on the node's own stream
+        where that is enough: a fork and its join cost a small backward pass 75 us of host time.  Enough means: nothing of this backward pass runs on the
+        weight-gradient stream yet, and what was added this way before was added on the same stream (a later fork waits for it: _issue_wgrad).  joined:
+        the node hands on a gradient, so that autograd makes the stream that backward() was called on wait for it."""
+        here = K.stream()
+        last = self._direct
+        if joined and not self._join_armed:
+            if last is None or last[0] != here:
+                now = torch.cuda.current_stream()
+                # (work from outside a capture is behind it already, and a captured stream may not wait for it)
+                if last is None or self._capturing(last[1]) != self._capturing(now):
+                    self._direct = last = (here, now)
+            if last is not None and last[0] == here:
+                fn()
+                return
+        self.on_wgrad_stream(fn, *tensors, tag=tag)
+
+    @staticmethod
+    def _capturing(stream) -> bool:
+        with torch.cuda.stream(stream):
+            return torch.cuda.is_current_stream_capturing()
+
+    def _behind_direct(self, s):
+        """`s` (None: the current stream) goes on behind what add_gradients launched on a node's own stream."""
+        (_, last), self._direct = self._direct, None
+        cur = torch.cuda.current_stream()
+        if last != cur and self._capturing(last) == self._capturing(cur):
+            (s if s is not None else cur).wait_stream(last)
+        if s is None:
+            self._direct = (cur.cuda_stream, cur)
+
     def _issue_wgrad(self, fn, tensors):
         s = self.wgrad_stream()
         if s is None:
+            if self._direct is not None:
+                self._behind_direct(None)
             self._in_wgrad = True
             try:
                 fn()
@@ -349,6 +384,8 @@ class Runtime:
         cur = torch.cuda.current_stream()
         if self.aux_stream is not None and self.text_stream is not None and cur == self.text_stream:
             s = self.adam_stream()
+        if self._direct is not None:
+            self._behind_direct(s)
         s.wait_stream(cur)
         self._override = s
         # fn() only launches kernels of this library: point them at the side stream directly instead of paying torch's

@@ -1,10 +1,13 @@
 """What keeps the packed operators inside their memory and their promises, without a GPU: the shares of the dK / dV pass compiled for the host."""
+import contextlib
 import os
 import random
 import re
 import subprocess
+import types
 
 import pytest
+import torch
 
 from crog_amd import _lib
 from crog_amd.packed import KEY_TILE, PackedRows
@@ -160,3 +163,118 @@ def test_requests_into_lds_hold_their_wait_states(tmp_path):
             waits += int(before.split()[1]) + 1 if before.startswith("s_nop") else 1
         assert moved
     assert requests > 500
+
+
+class Streams:
+    """Streams without a device: each knows which launches it comes behind."""
+
+    class One:
+        def __init__(self, handle, capturing=False):
+            self.cuda_stream, self.seen, self.capturing = handle, set(), capturing
+
+        def wait_stream(self, other):
+            assert self.capturing == other.capturing or not self.capturing, "a captured stream waits for work outside its capture"
+            self.seen |= other.seen
+
+    def __init__(self, monkeypatch, rt, defer=""):
+        from crog_amd import kernels as K
+        self.main, self.wgrad = self.One(1), self.One(99)
+        self.now, self.launched, self.callbacks, self.kept = self.main, [], [], []
+        self.all = {1: self.main, 99: self.wgrad}
+
+        @contextlib.contextmanager
+        def on(s):
+            old, self.now = self.now, s
+            yield
+            self.now = old
+        self.on = on
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: self.now)
+        monkeypatch.setattr(torch.cuda, "stream", on)
+        monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: self.now.capturing)
+        monkeypatch.setattr(torch.autograd.Variable, "_execution_engine", types.SimpleNamespace(queue_callback=self.callbacks.append))
+        monkeypatch.setattr(K, "stream", lambda: K._STREAM_OVERRIDE if K._STREAM_OVERRIDE is not None else self.now.cuda_stream)
+        monkeypatch.setattr(K, "gated_norm_bwd", lambda *a: self.slab())
+        monkeypatch.setattr(K, "gated_norm_sums", lambda slab, *a: self.launch(slab))
+        for name, value in (("_wgrad_stream", [self.wgrad]), ("_streams_ready", True), ("streams", [self.wgrad]), ("text_stream", None), ("aux_stream", None),
+                            ("_join_armed", False), ("_direct", None), ("defer_wgrad", defer), ("overlap_wgrad", True), ("deterministic", False)):
+            monkeypatch.setattr(rt, name, value, raising=False)
+        self.K = K
+
+    def user(self, handle, capturing=False):
+        return self.all.setdefault(handle, self.One(handle, capturing))
+
+    def slab(self):
+        slab = types.SimpleNamespace(record_stream=lambda s: None)
+        self.all[self.K.stream()].seen.add(id(slab))
+        self.kept.append(slab)
+        return slab
+
+    def launch(self, slab=None):
+        s = self.all[self.K.stream()]
+        assert slab is None or id(slab) in s.seen, "the sums are read before they are there"
+        for before in self.launched:
+            assert before in s.seen, "two kernels add onto one gradient, neither behind the other"
+        s.seen.add(len(self.launched))
+        self.launched.append(len(self.launched))
+
+    def end_of_backward(self, nodes_streams):
+        """backward() returns: its stream waits for the nodes whose gradients went on, and the queued callbacks run on it."""
+        for s in nodes_streams:
+            if s is not self.main:
+                self.main.wait_stream(s)
+        calls, self.callbacks[:] = list(self.callbacks), []
+        for c in calls:
+            c()
+        assert set(self.launched) <= self.main.seen, "backward() has returned, and its stream is not behind a weight's gradient"
+
+
+@pytest.mark.parametrize("defer", [""])
+@pytest.mark.parametrize("seed", range(40))
+def test_gradients_of_a_shared_weight_are_added_one_after_the_other(monkeypatch, seed, defer):
+    """Gated norms and LayerNorms that share a weight, their forward passes (so their backward nodes) on several streams of the user's: every addition onto the
+    weight's gradient is ordered against every other, and the stream that called backward() is behind them all."""
+    from crog_amd.functional import RT, GatedNormFn, WRef
+    from crog_amd.runtime import ParamStore
+    m = torch.nn.Module()
+    m.w = torch.nn.Parameter(torch.ones(8))
+    w = WRef(ParamStore(m, torch.device("cpu")), m.w, cols=1)
+    fake = Streams(monkeypatch, RT, defer)
+    rng = random.Random(seed)
+    x = torch.zeros(4, 8)
+    if rng.random() < 0.3:      # (the device's first stream may have been somebody else's before)
+        with fake.on(fake.user(7)):
+            GatedNormFn.backward(types.SimpleNamespace(cfg=(w, None, None, 1.0, False), saved_tensors=(x, x, x), needs_input_grad=(True, True)), x, None)
+        fake.end_of_backward([fake.user(7)])
+    for _ in range(3):
+        joined = []
+        for _ in range(rng.randrange(1, 6)):
+            s = rng.choice([fake.main, fake.main, fake.user(2), fake.user(3)])
+            with fake.on(s):
+                kind = rng.choice(["gated", "gated", "gated", "alone", "layer"])
+                if kind == "layer":
+                    RT.on_wgrad_stream(fake.launch, tag="ln")
+                else:
+                    needs = (False, False) if kind == "alone" else (True, rng.random() < 0.5)      # alone: only its weights take a gradient
+                    GatedNormFn.backward(types.SimpleNamespace(cfg=(w, None, None, 1.0, False), saved_tensors=(x, x, x), needs_input_grad=needs), x, None)
+                    if kind == "gated":
+                        joined.append(s)
+        fake.end_of_backward(joined)
+        for s in (fake.user(2), fake.user(3)):      # (the next forward pass on them begins behind the caller's stream)
+            s.wait_stream(fake.main)
+
+
+def test_a_capture_does_not_wait_for_gradients_added_before_it(monkeypatch):
+    from crog_amd.functional import RT
+    fake = Streams(monkeypatch, RT)
+    RT.add_gradients(fake.launch, joined=True)
+    captured = fake.user(5, capturing=True)
+    captured.seen |= fake.main.seen      # (a capture begins behind what was enqueued)
+    with fake.on(captured):
+        RT.add_gradients(fake.launch, joined=True)
+        fork = fake.user(6, capturing=True)
+        fork.wait_stream(captured)
+        fake.wgrad.capturing = True
+        with fake.on(fork):
+            RT.add_gradients(fake.launch, joined=True)
+    assert len(fake.launched) == 3 and len(fake.callbacks) == 1
