@@ -215,7 +215,7 @@ class Runtime:
         want = self.defer_wgrad == "all" or (self.defer_wgrad == "big" and defer)
         if want and self.overlap_wgrad and torch.cuda.is_available():
             self.flush_wgrad()
-            self._pending_wgrad.append((fn, tensors))
+            self._pending_wgrad.append((fn, tensors, torch.cuda.current_stream()))      # (the stream that its operands come from)
             if not self._join_armed:
                 try:
                     torch.autograd.Variable._execution_engine.queue_callback(self._end_of_backward)
@@ -227,8 +227,12 @@ class Runtime:
 
     def flush_wgrad(self):
         pend, self._pending_wgrad = self._pending_wgrad, []
-        for fn, tensors in pend:
-            self._issue_wgrad(fn, tensors)
+        for fn, tensors, *made_on in pend:
+            if made_on and made_on[0] != torch.cuda.current_stream():      # flushed by a node of another stream, or at the end of backward
+                with torch.cuda.stream(made_on[0]):
+                    self._issue_wgrad(fn, tensors)
+            else:
+                self._issue_wgrad(fn, tensors)
         done, self._pending_done = self._pending_done, []
         for d in done:
             d()

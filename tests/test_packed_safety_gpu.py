@@ -21,7 +21,7 @@ def store_of(seed=0, **shapes):
     return m, st, {n: WRef(st, p) if p.dim() == 2 else WRef(st, p, cols=1) for n, p in m.named_parameters()}
 
 
-@pytest.fixture(params=["as it is", "deterministic"])
+@pytest.fixture(params=["as it is", "deferred", "deterministic"])
 def mode(request):
     from crog_amd.runtime import RT, set_deterministic
     old = RT.defer_wgrad

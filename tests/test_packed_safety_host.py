@@ -229,7 +229,7 @@ class Streams:
         assert set(self.launched) <= self.main.seen, "backward() has returned, and its stream is not behind a weight's gradient"
 
 
-@pytest.mark.parametrize("defer", [""])
+@pytest.mark.parametrize("defer", ["", "all"])
 @pytest.mark.parametrize("seed", range(40))
 def test_gradients_of_a_shared_weight_are_added_one_after_the_other(monkeypatch, seed, defer):
     """Gated norms and LayerNorms that share a weight, their forward passes (so their backward nodes) on several streams of the user's: every addition onto the
