@@ -176,7 +176,10 @@ def is_mat(t: torch.Tensor) -> bool:
 
 def as_mat(t: torch.Tensor) -> torch.Tensor:
     """Return `t` if it is a valid row matrix view, else a contiguous copy (incoming autograd grads)."""
-    return t if is_mat(t) else t.contiguous()
+    if is_mat(t):
+        return t
+    t = t.contiguous()
+    return t if is_mat(t) else t.clone(memory_format=torch.contiguous_format)      # (a single row of any stride is contiguous to torch)
 
 
 # --------------------------------------------------------------------------------------------
@@ -766,9 +769,16 @@ def plan_used(plan):
         plan._table.record_stream(torch.cuda.current_stream())
 
 
+def _strides(t: torch.Tensor):
+    """Strides of [rows, heads, dim].  torch calls a tensor contiguous whatever stride a dimension of one element has: the kernels get that of a dense one."""
+    rows, heads, dim = t.shape
+    s0, s1, s2 = t.stride()
+    return (s0 if rows != 1 else heads * dim), (s1 if heads != 1 else dim), s2
+
+
 def heads16(t: torch.Tensor) -> torch.Tensor:
     """`t` [rows, heads, dim] if every head starts on a 16-byte boundary and its columns are adjacent, else a contiguous copy."""
-    s0, s1, s2 = t.stride()
+    s0, s1, s2 = _strides(t)
     vec = 16 // t.element_size()
     # (a tile of 64 rows is addressed with 32-bit offsets: rows or heads further apart than that are copied too)
     if s2 == 1 and s0 % vec == 0 and s1 % vec == 0 and t.data_ptr() % 16 == 0 and s0 < 1 << 22 and s1 * t.shape[1] < 1 << 27:
@@ -779,7 +789,7 @@ def heads16(t: torch.Tensor) -> torch.Tensor:
 
 def _heads(t: torch.Tensor):
     """(address, row stride, head stride) of a [rows, heads, dim] tensor"""
-    s = t.stride()
+    s = _strides(t)
     return t.data_ptr(), s[0], s[1]
 
 
@@ -808,13 +818,13 @@ def packed_attn_bwd(q, k, v, o, do, lse, D, dq, dk, dv, rows, scale):
 
 
 def rotary(q, k, q_out, k_out, positions, axes, inverse=False):
-    """q / k (either may be None): [rows, heads, dim] with adjacent columns; positions [rows, axes]; axes: packed.RotaryAxes."""
+    """q / k (either may be None): [rows, heads, dim] with adjacent columns; positions [rows, axes], contiguous; axes: packed.RotaryAxes."""
     t = q if q is not None else k
     plan_used(axes)
 
     none = (None, 0, 0)
     check(lib().crog_rotary(dcode(t), *(none if q is None else _heads(q)), *(none if k is None else _heads(k)), *(none if q is None else _heads(q_out)),
-                            *(none if k is None else _heads(k_out)), positions.data_ptr(), positions.stride(0),
+                            *(none if k is None else _heads(k_out)), positions.data_ptr(), axes.axes,
                             positions.element_size(), axes.revs_ptr, axes.axis_ptr, t.shape[0], 0 if q is None else q.shape[1],
                             0 if k is None else k.shape[1], t.shape[2], axes.pairs, axes.axes, axes.interleaved, inverse, stream()), "rotary")
 

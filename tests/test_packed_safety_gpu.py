@@ -161,3 +161,42 @@ def test_gated_norm_beside_the_frameworks_layers_captured_and_replayed():
         assert all(torch.equal(a, b) for a, b in zip(outs, want)), turn
         for n in r:
             assert torch.equal(r[n].grad(), once[n]) if n in norms else (r[n].grad() - once[n]).abs().max() <= 2.0 ** -14 * once[n].abs().max(), (turn, n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_one_row_and_one_head_of_any_stride(dtype):
+    """Slices of a cache or a projection with an odd or a very long stride along a dimension of one element."""
+    from crog_amd import functional as Fn
+    from crog_amd.packed import PackedRows, RotaryAxes
+
+    def odd(t, *strides):      # the same values, with these strides where t has one element
+        buf = torch.empty(max(t.numel() * 3, 4096), device="cuda", dtype=t.dtype)
+        return torch.as_strided(buf, t.shape, [s if n == 1 else d for n, s, d in zip(t.shape, strides, t.stride())]).copy_(t)
+    q, do = (dev(1, 1, 64, dtype=dtype, seed=i) for i in (1, 2))
+    k, v = (dev(300, 1, 64, dtype=dtype, seed=i) for i in (3, 4))
+    rows = PackedRows([1], [300], causal=True)
+
+    def grads(*ts):
+        leaves = [t.detach().requires_grad_() for t in ts[:3]]
+        o = Fn.packed_attention(*leaves, rows)
+        return [o.detach(), *torch.autograd.grad(o, leaves, ts[3])]
+    want = grads(q, k, v, do)
+    for s in ((260, 65), (1 << 24, 3), (7, 1 << 30)):
+        got = grads(odd(q, s[0], s[1], 1), odd(k, 0, s[1], 1), odd(v, 0, s[1], 1), odd(do, s[0], s[1], 1))
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), s
+    axes = RotaryAxes((8, 8, 16))
+    pos = torch.tensor([[5, 70, 900]], device="cuda")
+    a = Fn.rotary(q, k[:1], pos, axes)
+    for s in ((1, 1), (0, 1)):
+        b = Fn.rotary(odd(q, 65, 3, 1), odd(k[:1], 3, 5, 1), torch.as_strided(torch.cat([pos, pos]), (1, 3), s), axes)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    m, st, r = store_of(**WEIGHTS)
+    x, y = dev(1, C, dtype=dtype, seed=5), dev(1, C, dtype=dtype, seed=6)
+
+    def normed(x, y, g):
+        x, y = x.detach().requires_grad_(), y.detach().requires_grad_()
+        st.zero_grad()
+        u, h = Fn.gated_norm(x, y, post=(r["post_w"], r["post_b"]), gate=r["gate"], pre=(r["norm_w"], r["norm_b"]))
+        return [u.detach(), h.detach(), *torch.autograd.grad((u, h), (x, y), (g, g)), st.G.clone()]
+    want = normed(x, y, x)
+    assert all(torch.equal(a, b) for a, b in zip(normed(odd(x, 1, 1), odd(y, 3, 1), odd(x, 0, 1)), want))

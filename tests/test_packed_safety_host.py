@@ -278,3 +278,45 @@ def test_a_capture_does_not_wait_for_gradients_added_before_it(monkeypatch):
         with fake.on(fork):
             RT.add_gradients(fake.launch, joined=True)
     assert len(fake.launched) == 3 and len(fake.callbacks) == 1
+
+
+@pytest.mark.parametrize("shape,stride", [((3, 4, 64), (260, 65, 1)), ((1, 1, 64), (260, 65, 1)), ((1, 2, 128), (1 << 24, 128, 1)), ((5, 1, 64), (64, 3, 1)), ((1, 4, 64), (7, 64, 1)),
+                                          ((6, 1, 64), (128, 1 << 30, 1))])
+def test_heads_of_one_row_or_one_head_have_strides_the_kernels_take(shape, stride):
+    """torch leaves a dimension of one element whatever stride a slice gave it, and calls the tensor contiguous."""
+    from crog_amd import kernels as K
+    rows, heads, dim = shape
+    buf = torch.arange(rows * 600 + 600, dtype=torch.float32).bfloat16()
+    t = torch.as_strided(buf, shape, tuple(s if n > 1 else s for s, n in zip(stride, shape)))
+    got = K.heads16(t)
+    at, ld, hs = K._heads(got)
+    assert torch.equal(got, t) and at % 16 == 0 and ld % 8 == 0 and hs % 8 == 0 and 0 <= ld * 64 * 2 < 0x7fff0000 and 0 <= hs < 1 << 24
+    if rows * heads * dim and (heads == 1 or stride[1] % 8 == 0) and (rows == 1 or stride[0] % 8 == 0) and t.data_ptr() % 16 == 0:
+        assert got.data_ptr() == t.data_ptr()      # (nothing to copy)
+
+
+@pytest.mark.parametrize("shape,stride", [((1, 8), (1, 1)), ((1, 1, 8), (3, 5, 1)), ((4, 1, 8), (16, 2, 1)), ((1, 8), (0, 1)), ((3, 8), (0, 1)), ((2, 3, 8), (0, 8, 1))])
+def test_row_matrices_of_one_row_are_taken_whatever_its_stride(shape, stride):
+    from crog_amd import kernels as K
+    t = torch.as_strided(torch.arange(200.0), shape, stride)
+    m = K.as_mat(t)
+    rows, cols, ld = K.mat(m)
+    assert torch.equal(m, t) and (rows, cols) == (t.numel() // 8, 8) and ld >= 8
+    flat = torch.as_strided(m, (rows, cols), (ld, 1), m.storage_offset())
+    assert torch.equal(flat, t.reshape(rows, cols))
+
+
+@pytest.mark.parametrize("rows,axes,stride", [(1, 3, (1, 1)), (1, 1, (0, 1)), (1, 2, (0, 1)), (4, 2, (2, 1)), (4, 2, (7, 1)), (4, 2, (0, 1)), (4, 1, (3, 1)), (4, 1, (3, 5)), (1, 1, (0, 0))])
+def test_positions_of_one_row_or_one_axis_are_taken_whatever_their_strides(monkeypatch, rows, axes, stride):
+    from crog_amd import functional as Fn
+    from crog_amd import kernels as K
+    from crog_amd.packed import RotaryAxes
+    seen = {}
+    monkeypatch.setattr(K, "same_device", lambda *a: None)
+    monkeypatch.setattr(K, "plan_used", lambda a: None)
+    monkeypatch.setattr(K, "stream", lambda: 0)
+    names = _lib.parse_header()["crog_rotary"][2]
+    monkeypatch.setattr(K, "lib", lambda: types.SimpleNamespace(crog_rotary=lambda *a: seen.update(zip(names, a)) or 0))
+    pos = torch.as_strided(torch.arange(100), (rows, axes), stride)
+    Fn.rotary(torch.zeros(rows, 2, 16), None, pos, RotaryAxes((2,) * axes, device="cpu"))
+    assert seen["ldpos"] >= axes and seen["axes"] == axes and seen["rows"] == rows      # (what the C entry asks of them)
