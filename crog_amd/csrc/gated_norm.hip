@@ -13,6 +13,7 @@
 // over rows.  A thread holds at most 16 columns (four sums and four weights each are 128 registers): a row takes 16, 64, 256 or 512 threads.  Column sums: registers, then the block's groups through LDS, then one slab row per block, added up in block order by a
 // second launch - no atomics, the same bits every time.
 #include "common.h"
+#include <cmath>
 
 namespace {
 
@@ -412,6 +413,7 @@ extern "C" int crog_gated_norm_fwd(int dtype, const void* x, int64_t ldx, const 
                                    int rows, int cols, void* u, int64_t ldu, void* h, int64_t ldh, float* stats, crog_stream_t stream) {
   CROG_CHECK_ARG(dtype == CROG_F32 || dtype == CROG_BF16, "gated_norm_fwd: dtype must be CROG_F32 or CROG_BF16 (got %d)", dtype);
   CROG_CHECK_ARG(rows >= 0 && cols > 0 && cols <= MAX_COLS, "gated_norm_fwd: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
+  CROG_CHECK_ARG(std::isfinite(alpha), "gated_norm_fwd: alpha must be finite (got %g)", alpha);
   if (rows == 0) return CROG_OK;
   CROG_CHECK_ARG(x && y && u && (!has_pre || h) && ldx >= cols && ldy >= cols && ldu >= cols && (!has_pre || ldh >= cols), "gated_norm_fwd: bad tensors");
   CROG_CHECK_ARG((uintptr_t)stats % 16 == 0, "gated_norm_fwd: stats must be 16-byte aligned");
@@ -433,6 +435,7 @@ extern "C" int crog_gated_norm_bwd(int dtype, const void* x, int64_t ldx, const 
                                    crog_stream_t stream) {
   CROG_CHECK_ARG(dtype == CROG_F32 || dtype == CROG_BF16, "gated_norm_bwd: dtype must be CROG_F32 or CROG_BF16 (got %d)", dtype);
   CROG_CHECK_ARG(rows >= 0 && cols > 0 && cols <= MAX_COLS, "gated_norm_bwd: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
+  CROG_CHECK_ARG(std::isfinite(alpha), "gated_norm_bwd: alpha must be finite (got %g)", alpha);
   if (rows == 0) return CROG_OK;
   CROG_CHECK_ARG(x && y && stats && ldx >= cols && ldy >= cols && (!du || lddu >= cols) && (!dh || lddh >= cols) && (!dx || lddx >= cols) && (!dy || lddy >= cols),
                  "gated_norm_bwd: bad tensors");

@@ -13,6 +13,7 @@
 // half wave): the 16-byte slot of a row is XORed with the row's low bits, the lowest two moved to the slot's high bits.
 #include "gemm_dma.h"
 #include "packed_share.h"
+#include <cmath>
 #include <type_traits>
 
 namespace {
@@ -852,13 +853,14 @@ bool rows16(const void* p, int64_t ld, int64_t hs, int vec) { return ((uintptr_t
 // the rows of one tile lie within 2^31 bytes (32-bit offsets of the LDS requests)
 bool near(int64_t ld, int dtype) { return ld >= 0 && ld * 64 * (dtype == CROG_BF16 ? 2 : 4) < 0x7fff0000; }
 
-int check_common(const char* what, int dtype, int seqs, int rows_q, int rows_k, int kv_heads, int group, int head_dim, int n_tiles, const int* cu_q,
-                 const int* cu_k, const int* tiles) {
+int check_common(const char* what, int dtype, int seqs, int rows_q, int rows_k, int kv_heads, int group, int head_dim, float scale, int n_tiles,
+                 const int* cu_q, const int* cu_k, const int* tiles) {
   CROG_CHECK_ARG(dtype == CROG_F32 || dtype == CROG_BF16, "%s: dtype must be CROG_F32 or CROG_BF16 (got %d)", what, dtype);
   const int vec = dtype == CROG_BF16 ? 8 : 4;
   CROG_CHECK_ARG(head_dim > 0 && head_dim <= 128 && head_dim % vec == 0, "%s: head_dim must be a multiple of %d up to 128 (got %d)", what, vec, head_dim);
   CROG_CHECK_ARG(seqs > 0 && rows_q > 0 && rows_k > 0 && kv_heads > 0 && group > 0 && n_tiles >= 0, "%s: bad sizes", what);
   CROG_CHECK_ARG((int64_t)rows_q * group <= 0x7fffff00 && (int64_t)n_tiles * kv_heads <= 0x7fffffff && rows_k <= 0x7fffff00, "%s: too many rows", what);
+  CROG_CHECK_ARG(std::isfinite(scale * LOG2E), "%s: scale times log2(e) must be finite (got %g)", what, scale);
   CROG_CHECK_ARG(cu_q && cu_k && tiles, "%s: the sequence tables are missing", what);
   return CROG_OK;
 }
@@ -869,7 +871,7 @@ extern "C" int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64
                                     int64_t ldv, int64_t hsv, void* O, int64_t ldo, int64_t hso, float* lse, const int* cu_q, const int* cu_k,
                                     const int* tiles, int n_tiles, int seqs, int rows_q, int rows_k, int kv_heads, int group, int head_dim, float scale,
                                     int causal, int splits, int split_keys, float* partial, crog_stream_t stream) {
-  if (int rc = check_common("packed_attn_fwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_tiles, cu_q, cu_k, tiles)) return rc;
+  if (int rc = check_common("packed_attn_fwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, scale, n_tiles, cu_q, cu_k, tiles)) return rc;
   const int vec = dtype == CROG_BF16 ? 8 : 4;
   CROG_CHECK_ARG(rows16(Q, ldq, hsq, vec) && rows16(K, ldk, hsk, vec) && rows16(V, ldv, hsv, vec) && rows16(O, ldo, hso, vec) && Q && K && V && O,
                  "packed_attn_fwd: heads of Q / K / V / O must start at 16-byte boundaries");
@@ -908,8 +910,8 @@ extern "C" int crog_packed_attn_bwd(int dtype, const void* Q, int64_t ldq, int64
                                     const int* key_tiles, int n_key_tiles, int seqs, int rows_q, int rows_k, int kv_heads, int group, int head_dim,
                                     float scale, int causal, int splits, int split_keys, const int* key_units,
                                     int total_units, int share, float* partial, crog_stream_t stream) {
-  if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_row_tiles, cu_q, cu_k, row_tiles)) return rc;
-  if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, n_key_tiles, cu_q, cu_k, key_tiles)) return rc;
+  if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, scale, n_row_tiles, cu_q, cu_k, row_tiles)) return rc;
+  if (int rc = check_common("packed_attn_bwd", dtype, seqs, rows_q, rows_k, kv_heads, group, head_dim, scale, n_key_tiles, cu_q, cu_k, key_tiles)) return rc;
   const int vec = dtype == CROG_BF16 ? 8 : 4;
   CROG_CHECK_ARG(rows16(Q, ldq, hsq, vec) && rows16(K, ldk, hsk, vec) && rows16(V, ldv, hsv, vec) && rows16(O, ldo, hso, vec) && rows16(dO, lddo, hsdo, vec) &&
                  rows16(dQ, lddq, hsdq, vec) && rows16(dK, lddk, hsdk, vec) && rows16(dV, lddv, hsdv, vec) && Q && K && V && O && dO && lse && D && dQ && dK && dV,

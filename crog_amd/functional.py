@@ -1258,6 +1258,10 @@ def _fresh(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+MAX_FLOAT32 = torch.finfo(torch.float32).max
+MAX_SCALE = 2.358e38      # of attention: times log2(e) it is still a float32
+
+
 class PackedAttentionFn(Function):
     """o = softmax(scale q k^T) v within each sequence of a PackedRows plan (the packed form of the attention inside MhaFn: clip.py:246-260,
     layers.py:291-296,329-332), any head dim up to 128, grouped key heads."""
@@ -1308,7 +1312,7 @@ def packed_attention(q, k, v, rows, scale=None):
     # (one condition for the calls that are right; what is wrong with another is found out behind it)
     if not (len(qs) == 3 == len(ks) and ks == v.shape and k.dtype == dt == v.dtype and qs[2] == ks[2] and qs[1] == ks[1] * group and ks[1] > 0
             and 0 < qs[2] <= 128 and qs[2] % (16 // q.element_size()) == 0 and qs[0] >= rows.rows_q and ks[0] >= rows.rows_k
-            and (dt is torch.bfloat16 or dt is torch.float32) and (scale is None or math.isfinite(scale))):
+            and (dt is torch.bfloat16 or dt is torch.float32) and (scale is None or abs(scale) <= MAX_SCALE)):
         _refuse_attention(q, k, v, rows, scale)
     K.same_device(q, k, v, rows._table)
     return PackedAttentionFn.apply(q, k, v, rows, qs[2] ** -0.5 if scale is None else float(scale))
@@ -1328,7 +1332,7 @@ def _refuse_attention(q, k, v, rows, scale):
         raise ValueError(f"packed_attention: the head dimension must be a multiple of {vec} up to 128 for {q.dtype}, got {dim}")
     if q.shape[0] < rows.rows_q or k.shape[0] < rows.rows_k:
         raise ValueError(f"packed_attention: the plan has {rows.rows_q} query and {rows.rows_k} key rows, the tensors {q.shape[0]} and {k.shape[0]}")
-    raise ValueError(f"packed_attention: scale must be finite, got {scale}")
+    raise ValueError(f"packed_attention: scale must be finite, also as a float32 in units of log 2 (at most {MAX_SCALE}), got {scale}")
 
 
 class RotaryFn(Function):
@@ -1451,8 +1455,8 @@ def gated_norm(x, y, *, post=None, gate: Optional[WRef] = None, pre=None, res_sc
     for r in refs:
         if r.rows * r.cols != C:
             raise ValueError(f"gated_norm: a weight of {r.rows * r.cols} values for rows of {C} columns")
-    if not eps >= 0 or not math.isfinite(res_scale):
-        raise ValueError("gated_norm: eps must not be negative and res_scale must be finite")
+    if not eps >= 0 or not abs(res_scale) <= MAX_FLOAT32:
+        raise ValueError("gated_norm: eps must not be negative and res_scale must be finite, also as a float32")
     K.same_device(x, y, *{id(r.P): r.P for r in refs}.values())
     return GatedNormFn.apply(K.as_mat(x), K.as_mat(y), gate, post, pre, float(res_scale), float(eps), bool(rms), *[r.param for r in refs])
 

@@ -320,3 +320,34 @@ def test_positions_of_one_row_or_one_axis_are_taken_whatever_their_strides(monke
     pos = torch.as_strided(torch.arange(100), (rows, axes), stride)
     Fn.rotary(torch.zeros(rows, 2, 16), None, pos, RotaryAxes((2,) * axes, device="cpu"))
     assert seen["ldpos"] >= axes and seen["axes"] == axes and seen["rows"] == rows      # (what the C entry asks of them)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 2.4e38, -3.4e38, 1e308])
+def test_scales_that_float32_does_not_hold_are_refused(scale):
+    """The kernels take the scale in float32 and in units of log 2: beyond that range every score would be an infinity or NaN."""
+    from crog_amd import functional as Fn
+    q = torch.zeros(6, 2, 64)
+    rows = PackedRows([6], device="cpu")
+    with pytest.raises(ValueError):
+        Fn.packed_attention(q, q, q, rows, scale)
+    with pytest.raises(RuntimeError):      # (all well: but there is no CPU path)
+        Fn.packed_attention(q, q, q, rows, scale / 1e308)
+    if abs(scale) > 3.5e38:
+        with pytest.raises(ValueError):
+            Fn.gated_norm(torch.zeros(4, 8), torch.zeros(4, 8), res_scale=scale)
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan"), 3e38])
+def test_c_entries_refuse_scales_that_are_not_finite(value):
+    lib = _lib.load()
+    buf = torch.zeros(4096)
+    p = (buf.data_ptr() + 15) // 16 * 16
+    fwd = [1] + [p, 64, 64] * 4 + [None, p, p, p, 1, 1, 8, 8, 1, 1, 64, value, 0, 1, 0, None, None]
+    bwd = [1] + [p, 64, 64] * 5 + [p, p] + [p, 64, 64] * 3 + [p, p, p, 1, p, 1, 1, 8, 8, 1, 1, 64, value, 0, 1, 0, None, 0, 0, None, None]
+    calls = [(lib.crog_packed_attn_fwd, fwd), (lib.crog_packed_attn_bwd, bwd)]
+    if value != 3e38:      # (a float32 like any other where no logarithm is taken)
+        calls += [(lib.crog_gated_norm_fwd, [1, p, 64, p, 64, None, None, None, None, None, 0, 1, 0, value, 1e-5, 0, 64, p, 64, p, 64, None, None]),
+                  (lib.crog_gated_norm_bwd, [1, p, 64, p, 64, p, 64, p, 64, None, None, None, None, 0, 1, 0, value, 0, 64, p, p, 64, p, 64, None, None])]
+    for entry, args in calls:
+        assert len(args) == len(entry.argtypes)
+        assert entry(*args) == -1 and b"finite" in lib.crog_last_error()
