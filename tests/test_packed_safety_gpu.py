@@ -200,3 +200,132 @@ def test_one_row_and_one_head_of_any_stride(dtype):
         return [u.detach(), h.detach(), *torch.autograd.grad((u, h), (x, y), (g, g)), st.G.clone()]
     want = normed(x, y, x)
     assert all(torch.equal(a, b) for a, b in zip(normed(odd(x, 1, 1), odd(y, 3, 1), odd(x, 0, 1)), want))
+
+
+def test_a_dropped_plan_keeps_its_memory_until_its_launches_have_read_it():
+    """Plans made on one stream, used on another that is still busy, and dropped: their tables' memory goes to no new tensor before the launches on the other
+    stream are through."""
+    import weakref
+
+    from crog_amd import functional as Fn
+    from crog_amd.packed import PackedRows, RotaryAxes
+    lens = [400, 100]
+    q, k, v, do = (dev(500, 2, 64, dtype=torch.bfloat16, seed=i) for i in range(4))
+    pos = torch.arange(500, device="cuda")
+
+    def run(rows, axes):
+        a, b, c = (t.detach().requires_grad_() for t in (q, k, v))
+        o = Fn.packed_attention(*Fn.rotary(a, b, pos, axes), c, rows)
+        return [o.detach().clone(), *torch.autograd.grad(o, (a, b, c), do)]
+
+    def plans():
+        return PackedRows(lens, causal=True), RotaryAxes((32,))
+    want = run(*plans())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(*plans())      # (what a first pass allocates on that stream is there)
+    torch.cuda.synchronize()
+    sizes = [p._table.numel() * p._table.element_size() for p in plans()]
+
+    def fillers():      # (new memory of the tables' size classes, on the stream that the plans were made on; kept, so that each is another)
+        return [torch.full((n,), 255, device="cuda", dtype=torch.uint8) for n in sizes for _ in range(40)]
+    # without a launch the memory is given away at once: fillers do come to lie where the tables lay
+    rows, axes = plans()
+    tables = {rows._table.data_ptr(), axes._table.data_ptr()}
+    del rows, axes
+    assert tables <= {t.data_ptr() for t in fillers()}
+
+    rows, axes = plans()
+    tables, alive = {rows._table.data_ptr(), axes._table.data_ptr()}, [weakref.ref(rows), weakref.ref(axes)]
+    work = torch.randn(4096, 4096, device="cuda")
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(150):      # (a tenth of a second of work ahead of the launches)
+            work = torch.mm(work, work) * 1e-2
+        got = run(rows, axes)
+        done = side.record_event()
+    del rows, axes
+    dropped = not any(r() for r in alive)
+    new = fillers()
+    busy = not done.query()
+    torch.cuda.synchronize()
+    assert dropped
+    assert busy, "the other stream was through before the fillers were made: the test shows nothing"
+    assert not tables & {t.data_ptr() for t in new}
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def within(got, want, bound, what):
+    off = (got.double() - want).abs()
+    worst = (off / bound.clamp_min(1e-300)).max().item()
+    assert (off <= bound).all(), f"{what}: off by {worst:.3g} times its bound"
+
+
+@pytest.mark.parametrize("n,causal,group,tight", [(65, True, 1, "dq dv"), (100, False, 1, "dq dv"), (128, True, 1, "dq dv"), (128, False, 2, "dv"), (64, False, 2, "dq dv"),
+                                                  (129, False, 1, ""), (129, True, 1, "")])
+def test_attention_gradients_on_both_sides_of_the_few_row_rule(n, causal, group, tight):
+    """Up to 128 rows (dQ: queries times group; dK / dV: queries) the rests of the rounded probabilities and dS follow them.  Bounds, added up from the
+    roundings: the output by half a step, a rest by half a step of half a step (2^-16; a rounded value alone 2^-8), D = dO . o from the stored o (half a step of
+    o), the probabilities by float32 arithmetic (2^-24 for each of the 64 terms of a score and the n terms of a sum, worst case, as relative error)."""
+    from crog_amd import functional as Fn
+    from crog_amd.packed import PackedRows
+    D, h, U = 64, 2.0 ** -8, 2.0 ** -24
+    lens = [n] * 3
+    rows = PackedRows(lens, group=group, causal=causal)
+    q, do = (dev(3 * n, group, D, dtype=torch.bfloat16, seed=i).requires_grad_(i == 1) for i in (1, 2))
+    k, v = (dev(3 * n, 1, D, dtype=torch.bfloat16, seed=i).requires_grad_() for i in (3, 4))
+    dq, dk, dv = torch.autograd.grad(Fn.packed_attention(q, k, v, rows), (q, k, v), do)
+    ok = torch.ones(n, n, dtype=torch.bool, device="cuda")
+    ok = ok.tril() if causal else ok
+    for s in range(3):
+        at = slice(s * n, (s + 1) * n)
+        kk, vv = k[at, 0].detach().double(), v[at, 0].detach().double()
+        want_v = torch.zeros(n, D, dtype=torch.float64, device="cuda")
+        err_v = torch.zeros_like(want_v)
+        for g in range(group):
+            qq, gg = q[at, g].detach().double(), do[at, g].double()
+            x = qq @ kk.T / 8
+            p = torch.softmax(x.masked_fill(~ok, -float("inf")), 1)
+            o, dp = p @ vv, gg @ vv.T
+            ep = 2 * U * ((D + 4) * (qq.abs() @ kk.abs().T / 8).amax(1, keepdim=True) + 16) + U * n
+            rest = h * h if "dv" in tight else h
+            want_v += p.T @ gg
+            err_v += (p * (rest + ep)).T @ gg.abs() + U * (n * group + 4) * (p.T @ gg.abs())
+            ds = p * (dp - (gg * o).sum(1, keepdim=True)) / 8
+            stored = h * o.abs() + (h + ep) * (p @ vv.abs()) * (1 + h)      # (the forward's probabilities are rounded without a rest)
+            edd = (gg.abs() * stored).sum(1, keepdim=True) + U * (D + n) * (gg.abs() @ vv.abs().T).amax(1, keepdim=True)
+            rest = h * h if "dq" in tight else h
+            eds = p / 8 * (edd + U * (D + 4) * (gg.abs() @ vv.abs().T)) + ds.abs() * (rest + ep + 4 * U)
+            want_q = ds @ kk
+            within(dq[at, g], want_q, (h * want_q.abs() + (eds @ kk.abs() + U * n * (ds.abs() @ kk.abs())) * (1 + h)), f"dq of sequence {s}")
+        within(dv[at, 0], want_v, h * want_v.abs() + err_v * (1 + h), f"dv of sequence {s}")
+
+
+@pytest.mark.parametrize("n,group", [(100, 1), (128, 1), (64, 2), (65, 1)])
+def test_dq_of_few_rows_carries_the_rests(n, group):
+    """As above, with D from the o that the forward stored where a row sees more than one tile of 64 keys (what the kernel takes), so that its rounding is no
+    part of the bound: what is left is the output's half step, the rests' 2^-16 and float32 arithmetic."""
+    from crog_amd import functional as Fn
+    from crog_amd.packed import PackedRows
+    D, h, U = 64, 2.0 ** -8, 2.0 ** -24
+    rows = PackedRows([n] * 3, group=group)
+    q, do = (dev(3 * n, group, D, dtype=torch.bfloat16, seed=i).requires_grad_(i == 1) for i in (1, 2))
+    k, v = (dev(3 * n, 1, D, dtype=torch.bfloat16, seed=i) for i in (3, 4))
+    o = Fn.packed_attention(q, k, v, rows)
+    dq, = torch.autograd.grad(o, q, do)
+    for s in range(3):
+        at = slice(s * n, (s + 1) * n)
+        kk, vv = k[at, 0].double(), v[at, 0].double()
+        for g in range(group):
+            qq, gg = q[at, g].detach().double(), do[at, g].double()
+            p = torch.softmax(qq @ kk.T / 8, 1)
+            ep = 2 * U * ((D + 4) * (qq.abs() @ kk.abs().T / 8).amax(1, keepdim=True) + 16) + U * n
+            oo = o[at, g].detach().double() if n > 64 else p @ vv
+            dp = gg @ vv.T
+            ds = p * (dp - (gg * oo).sum(1, keepdim=True)) / 8
+            want = ds @ kk
+            edd = U * (D + n) * ((gg.abs() * oo.abs()).sum(1, keepdim=True) + (p * dp.abs()).sum(1, keepdim=True))
+            edd = edd + (gg.abs() * ep * (p @ vv.abs())).sum(1, keepdim=True) * (n <= 64)
+            eds = p / 8 * (edd + U * (D + 4) * (gg.abs() @ vv.abs().T)) + ds.abs() * (h * h + ep + 4 * U)
+            within(dq[at, g], want, h * want.abs() + (eds @ kk.abs() + U * n * (ds.abs() @ kk.abs())) * (1 + h), f"dq of sequence {s}")
