@@ -412,7 +412,7 @@ extern "C" int crog_gated_norm_fwd(int dtype, const void* x, int64_t ldx, const 
                                    const float* post_b, const float* pre_w, const float* pre_b, int has_post, int has_pre, int rms, float alpha, float eps,
                                    int rows, int cols, void* u, int64_t ldu, void* h, int64_t ldh, float* stats, crog_stream_t stream) {
   CROG_CHECK_ARG(dtype == CROG_F32 || dtype == CROG_BF16, "gated_norm_fwd: dtype must be CROG_F32 or CROG_BF16 (got %d)", dtype);
-  CROG_CHECK_ARG(rows >= 0 && cols > 0 && cols <= MAX_COLS, "gated_norm_fwd: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
+  CROG_CHECK_ARG(rows >= 0 && rows <= 0x7fff0000 && cols > 0 && cols <= MAX_COLS, "gated_norm_fwd: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
   CROG_CHECK_ARG(std::isfinite(alpha), "gated_norm_fwd: alpha must be finite (got %g)", alpha);
   if (rows == 0) return CROG_OK;
   CROG_CHECK_ARG(x && y && u && (!has_pre || h) && ldx >= cols && ldy >= cols && ldu >= cols && (!has_pre || ldh >= cols), "gated_norm_fwd: bad tensors");
@@ -434,7 +434,7 @@ extern "C" int crog_gated_norm_bwd(int dtype, const void* x, int64_t ldx, const 
                                    int rms, float alpha, int rows, int cols, const float* stats, void* dx, int64_t lddx, void* dy, int64_t lddy, float* slab,
                                    crog_stream_t stream) {
   CROG_CHECK_ARG(dtype == CROG_F32 || dtype == CROG_BF16, "gated_norm_bwd: dtype must be CROG_F32 or CROG_BF16 (got %d)", dtype);
-  CROG_CHECK_ARG(rows >= 0 && cols > 0 && cols <= MAX_COLS, "gated_norm_bwd: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
+  CROG_CHECK_ARG(rows >= 0 && rows <= 0x7fff0000 && cols > 0 && cols <= MAX_COLS, "gated_norm_bwd: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
   CROG_CHECK_ARG(std::isfinite(alpha), "gated_norm_bwd: alpha must be finite (got %g)", alpha);
   if (rows == 0) return CROG_OK;
   CROG_CHECK_ARG(x && y && stats && ldx >= cols && ldy >= cols && (!du || lddu >= cols) && (!dh || lddh >= cols) && (!dx || lddx >= cols) && (!dy || lddy >= cols),
@@ -455,7 +455,7 @@ extern "C" int crog_gated_norm_bwd(int dtype, const void* x, int64_t ldx, const 
 
 extern "C" int crog_gated_norm_sums(const float* slab, int rows, int cols, const float* gate, const float* post_w, const float* post_b, int has_post,
                                     float* dgate, float* dpost_w, float* dpost_b, float* dpre_w, float* dpre_b, crog_stream_t stream) {
-  CROG_CHECK_ARG(rows >= 0 && cols > 0 && cols <= MAX_COLS, "gated_norm_sums: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
+  CROG_CHECK_ARG(rows >= 0 && rows <= 0x7fff0000 && cols > 0 && cols <= MAX_COLS, "gated_norm_sums: rows of 1 .. %d columns (got %d x %d)", MAX_COLS, rows, cols);
   if (rows == 0 || !(dgate || dpost_w || dpost_b || dpre_w || dpre_b)) return CROG_OK;
   CROG_CHECK_ARG(slab, "gated_norm_sums: the slab of crog_gated_norm_bwd is missing");
   gated_norm_sums_kernel<<<cdiv(cols, 16), 16 * RUNS, 0, (hipStream_t)stream>>>(slab, blocks_for(rows, cols), cols, gate, post_w, post_b, has_post, dgate,

@@ -118,7 +118,7 @@ extern "C" int crog_rotary(int dtype, const void* Q, int64_t ldq, int64_t hsq, c
                            const int* axis, int rows, int heads_q, int heads_k, int head_dim, int pairs, int axes, int interleaved, int inverse,
                            crog_stream_t stream) {
   CROG_CHECK_ARG(dtype == CROG_F32 || dtype == CROG_BF16, "rotary: dtype must be CROG_F32 or CROG_BF16 (got %d)", dtype);
-  CROG_CHECK_ARG(rows >= 0 && heads_q >= 0 && heads_k >= 0 && (int64_t)(heads_q + heads_k) * head_dim <= (1 << 24), "rotary: bad sizes");
+  CROG_CHECK_ARG(rows >= 0 && rows <= 0x7fff0000 && heads_q >= 0 && heads_k >= 0 && (int64_t)(heads_q + heads_k) * head_dim <= (1 << 24), "rotary: bad sizes");
   CROG_CHECK_ARG(pairs > 0 && pairs <= MAXP && 2 * pairs <= head_dim, "rotary: 2 * pairs must fit the head and pairs be at most %d (pairs %d, head_dim %d)",
                  MAXP, pairs, head_dim);
   if (rows == 0 || heads_q + heads_k == 0) return CROG_OK;

@@ -1259,6 +1259,7 @@ def _fresh(t: torch.Tensor) -> torch.Tensor:
 
 
 MAX_FLOAT32 = torch.finfo(torch.float32).max
+MAX_ROWS = 0x7fff0000      # the kernels' row numbers have 32 bits, with room for a block's step behind the last
 MAX_SCALE = 2.358e38      # of attention: times log2(e) it is still a float32
 
 
@@ -1369,6 +1370,8 @@ def rotary(q, k, positions, axes):
     ([rows] for one axis), as `axes` (packed.RotaryAxes) says; -> (q', k').  Columns behind the plan's pairs are copied."""
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
         raise ValueError(f"rotary: q and k must be [rows, heads, dim] with the same rows and dim, got {tuple(q.shape)}, {None if k is None else tuple(k.shape)}")
+    if q.shape[0] > MAX_ROWS:
+        raise ValueError(f"rotary: {q.shape[0]} rows are too many")
     K.dcode(q)
     if k is not None and k.dtype != q.dtype:
         raise TypeError(f"rotary: q and k must have one dtype, got {q.dtype} and {k.dtype}")
@@ -1442,6 +1445,8 @@ def gated_norm(x, y, *, post=None, gate: Optional[WRef] = None, pre=None, res_sc
     C = x.shape[-1]
     if not 0 < C <= 8192:
         raise ValueError(f"gated_norm: rows of 1 to 8192 columns, got {C}")
+    if x.numel() > MAX_ROWS * C:
+        raise ValueError(f"gated_norm: {x.numel() // C} rows are too many")
     refs = [gate]
     for name, w in (("post", post), ("pre", pre)):
         if w is None:

@@ -152,7 +152,10 @@ class RotaryAxes:
         if not (theta > 0):
             raise ValueError("RotaryAxes: theta must be positive")
         self.axes, self.pairs, self.interleaved, self.theta = len(sizes), sum(sizes), bool(interleaved), float(theta)
-        revs = np.concatenate([float(theta) ** (-np.arange(n, dtype=np.float64) / n) for n in sizes]) / (2 * np.pi)
+        with np.errstate(over="ignore"):
+            revs = np.concatenate([float(theta) ** (-np.arange(n, dtype=np.float64) / n) for n in sizes]) / (2 * np.pi)
+        if not np.isfinite(revs).all():
+            raise ValueError(f"RotaryAxes: theta {theta} gives angles beyond 64 bits")
         axis = np.repeat(np.arange(len(sizes), dtype=np.int64), sizes).astype(np.int32)
         raw = np.concatenate([revs.view(np.uint8), axis.view(np.uint8)])      # (the doubles first: aligned)
         self._table = torch.from_numpy(raw).to(device)

@@ -351,3 +351,33 @@ def test_c_entries_refuse_scales_that_are_not_finite(value):
     for entry, args in calls:
         assert len(args) == len(entry.argtypes)
         assert entry(*args) == -1 and b"finite" in lib.crog_last_error()
+
+
+@pytest.mark.parametrize("rows", [(1 << 32) + 5, 1 << 31, 0x7fff0001])
+def test_more_rows_than_the_kernels_count_are_refused(rows):
+    """Row numbers are 32 bits on the device: 2^32 + 5 rows would be taken for five."""
+    from crog_amd import functional as Fn
+    from crog_amd.packed import RotaryAxes
+    x = torch.zeros(1, 8).expand(rows, 8)
+    with pytest.raises(ValueError, match="rows"):
+        Fn.gated_norm(x, x)
+    with pytest.raises(ValueError, match="rows"):
+        Fn.gated_norm(x[None], x[None])
+    q, pos = torch.zeros(1, 1, 4).expand(rows, 1, 4), torch.zeros(1, dtype=torch.int32).expand(rows)
+    with pytest.raises(ValueError, match="rows"):
+        Fn.rotary(q, None, pos, RotaryAxes((2,), device="cpu"))
+    lib = _lib.load()
+    if rows < 1 << 31:
+        buf = torch.zeros(4096)
+        p = (buf.data_ptr() + 15) // 16 * 16
+        assert lib.crog_rotary(1, p, 64, 64, p, 64, 64, p, 64, 64, p, 64, 64, p, 1, 4, p, p, rows, 1, 1, 64, 32, 1, 0, 0, None) == -1
+        assert lib.crog_gated_norm_fwd(1, p, 64, p, 64, None, None, None, None, None, 0, 1, 0, 1.0, 1e-5, rows, 64, p, 64, p, 64, None, None) == -1
+        assert lib.crog_gated_norm_bwd(1, p, 64, p, 64, p, 64, p, 64, None, None, None, None, 0, 1, 0, 1.0, rows, 64, p, p, 64, p, 64, None, None) == -1
+
+
+def test_a_theta_whose_angles_overflow_is_refused():
+    """A position of zero times an infinite angle is NaN."""
+    from crog_amd.packed import RotaryAxes
+    with pytest.raises(ValueError, match="theta"):
+        RotaryAxes((128,), theta=5e-324, device="cpu")
+    RotaryAxes((128,), theta=1e-300, device="cpu")
