@@ -769,27 +769,24 @@ def plan_used(plan):
         plan._table.record_stream(torch.cuda.current_stream())
 
 
-def _strides(t: torch.Tensor):
-    """Strides of [rows, heads, dim].  torch calls a tensor contiguous whatever stride a dimension of one element has: the kernels get that of a dense one."""
-    rows, heads, dim = t.shape
-    s0, s1, s2 = t.stride()
-    return (s0 if rows != 1 else heads * dim), (s1 if heads != 1 else dim), s2
-
-
 def heads16(t: torch.Tensor) -> torch.Tensor:
     """`t` [rows, heads, dim] if every head starts on a 16-byte boundary and its columns are adjacent, else a contiguous copy."""
-    s0, s1, s2 = _strides(t)
+    s0, s1, s2 = t.stride()
     vec = 16 // t.element_size()
     # (a tile of 64 rows is addressed with 32-bit offsets: rows or heads further apart than that are copied too)
     if s2 == 1 and s0 % vec == 0 and s1 % vec == 0 and t.data_ptr() % 16 == 0 and s0 < 1 << 22 and s1 * t.shape[1] < 1 << 27:
         return t
+    rows, heads, dim = t.shape
+    if rows == 1 and s0 != heads * dim or heads == 1 and s1 != dim:
+        # a dimension of one element has any stride (and is contiguous to torch whatever it is): that of a dense tensor will do
+        return heads16(t.as_strided(t.shape, (s0 if rows != 1 else heads * dim, s1 if heads != 1 else dim, s2)))
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _heads(t: torch.Tensor):
     """(address, row stride, head stride) of a [rows, heads, dim] tensor"""
-    s = _strides(t)
+    s = t.stride()
     return t.data_ptr(), s[0], s[1]
 
 
