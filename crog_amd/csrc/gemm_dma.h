@@ -20,7 +20,8 @@ constexpr unsigned DMA_OOB = 0x80000000u;
 #ifndef CROG_ASM_DMA
 #define CROG_ASM_DMA 1
 #endif
-// The text holds the wait state that the hardware wants between the write of M0 and a load that goes to LDS by it (the compiler's own such pairs have it).
+// The text holds the wait state that the hardware wants between the write of M0 and a load that goes to LDS by it (the compiler's own such pairs have it;
+// the CROG training step took 27.24 ms without, 27.31 with).
 typedef int dma_i32x4 __attribute__((ext_vector_type(4)));
 __device__ __attribute__((always_inline)) inline void dma_piece(const void* base, int extent, char* dst, unsigned off) {
 #ifdef CROG_PROBE_NO_OOB      // probe build (LAB_NOTES section 10): no lane is ever out of range - border taps read the operand's first bytes (WRONG values, on purpose)

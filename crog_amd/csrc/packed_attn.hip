@@ -11,6 +11,9 @@
 // products; its k index is the lane's half, so the registers are that operand as they stand.
 // One LDS image serves both ways of reading a tile - rows (16 bytes a lane, lane = row) and columns (ds_read_b64_tr_b16, four rows x 64 bytes a
 // half wave): the 16-byte slot of a row is XORed with the row's low bits, the lowest two moved to the slot's high bits.
+// Requests into LDS and their waits are assembly, so the compiler does not know when the resident operands (ordinary loads: qf, gf, kf, vf) have arrived.
+// It guards their first use with a wait of its own, and that use stands inside each main loop, behind the request for a tile ahead: as compiled, every
+// loop waits for what it has just requested (forward vmcnt(0), dQ vmcnt(1), dK / dV vmcnt(0), at 128 bf16 columns vmcnt(5)) before its first product.
 #include "gemm_dma.h"
 #include "packed_share.h"
 #include <cmath>
@@ -243,10 +246,12 @@ template <typename T, int DP, int R> struct Fetch {
 
 // =====================================================================================================================
 // forward.  grid (kv_heads * tiles, key splits); a block owns 128 rows of one sequence and key head, keys stream through LDS in two buffers of 64.
-// Bound: at 128 columns the matrix units (one causal sequence of 16384 rows, 16 / 2 heads: 1045 us, 1.05 PFLOP/s; a large library product reaches 1.24
-// here), at 64 the vector work of the softmax beside them (a maximum, a fused step, an exponential, a sum and a conversion an element: 32 sequences of
-// 676 tokens, 8 heads: 50 us, 0.6 PFLOP/s), for single tokens memory (16 sequences of 200 to 8192 keys, 32 / 8 heads of 128: 71 + 5 us, 4.0 TB/s).  64
-// rows a wave instead of 32, one wave a SIMD: 1370 us for the long sequence.
+// Measured: one causal sequence of 16384 rows, 16 / 2 heads of 128: 1060 us, 1.04 PFLOP/s (a large library product reaches 1.24 here), at 1.9 GHz the matrix
+// units busy 50 % of the clocks, the vector units 46 %; 32 sequences of 676 tokens, 8 heads of 64: 51 us, 0.6 PFLOP/s, matrix 25 %, vector 48 % (a maximum,
+// a fused step, an exponential, a sum and a conversion an element).  Bound by neither unit alone but by one waiting for the other and both for the tile
+// that each step has just requested (the waves wait 29 and 37 % of their time).  Single tokens (16 sequences of 200 to 8192 keys, 32 / 8 heads of 128:
+// 71 + 5 us, 4.0 TB/s) wait for memory with nothing else in flight; with at most 32 rows one wave of four has products, the others fetch only.  64 rows a
+// wave instead of 32, one wave a SIMD: 1370 us for the long sequence.  P is rounded to bf16 for the second product (mma_cols), the sum is of the float P.
 // =====================================================================================================================
 template <typename T, int DP, int DC, int NB>
 __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
@@ -390,8 +395,8 @@ __global__ void __launch_bounds__(NT, 2) packed_fwd_kernel(const PackedArgs a) {
 }
 
 // the splits of a row meet: o = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.  W waves of a row take every W-th split each (W = 4 from 8 splits on: one
-// row of 63 splits took 21.7 us on one wave); a lane takes the statistics of one of its wave's splits, so that their loads, and after that those of
-// the partial rows, are in flight together.
+// row of 63 splits took 21.7 us on one wave); a lane takes the statistics of one of its wave's splits, so that their loads are in flight together.  The
+// partial rows come one behind the other (the compiler does not unroll a loop of unknown length around a read of another lane).
 template <typename T, int W>
 __global__ void __launch_bounds__(NT) packed_combine_kernel(const PackedArgs a, int splits) {
   constexpr int ROWS = 4 / W;
@@ -427,7 +432,6 @@ __global__ void __launch_bounds__(NT) packed_combine_kernel(const PackedArgs a, 
     sum += f * l;
     const int n = live ? min(64, (splits - z0 + W - 1) / W) : 0;
     const float* p = a.part_o + (z0 * total + row) * a.dim;
-#pragma unroll 8
     for (int z = 0; z < n; z++) {
       const float fz = readlane_f(f, z);
       o0 += fz * p[z * W * total * a.dim + c0];
@@ -463,7 +467,9 @@ void launch_combine(const PackedArgs& a, int splits, int64_t total, hipStream_t 
 
 // =====================================================================================================================
 // backward 1: D and dQ, blocked as the forward, its few rows over long keys cut in the same way (the float sums meet in packed_dq_sum_kernel).  Three
-// products a tile: 1.1 PFLOP/s at 128 columns (four sequences of 4096 rows, 16 / 4 heads: 730 us), 0.66 at 64 (32 of 676 tokens, 8 heads: 68 us).
+// products a tile, of which S and dP are formed again by the next kernel (nine in all with the forward's, where seven are needed): counting all three,
+// 1.1 PFLOP/s at 128 columns (four sequences of 4096 rows, 16 / 4 heads: 730 us), 0.66 at 64 (32 of 676 tokens, 8 heads: 69 us; matrix units busy 29 %,
+// vector units 41 % of the clocks).  P and dS are rounded to bf16 for their products.  float: 17 registers spilled at 128 columns, two at 96.
 // =====================================================================================================================
 template <typename T, int DP, int DC, int NB>
 __global__ void __launch_bounds__(NT, sizeof(T) == 2 && DC <= 32 ? 4 : 2) packed_bwd_dq_kernel(const PackedArgs a) {
@@ -615,13 +621,14 @@ __global__ void __launch_bounds__(NT) packed_dq_sum_kernel(const PackedArgs a, i
 
 // =====================================================================================================================
 // backward 2: dK, dV.  A block takes 128 keys at a time, 32 a wave, and the group's query rows stream past them through a ring of four LDS tiles of
-// 32 rows, requested three steps ahead.
+// 32 rows, requested three steps ahead (of which the compiler's wait, see the top, leaves the step's own request: the counted waits below never bind).
+// bf16 at 128 columns: seven registers spilled, two of them read back in the partial form of the request, which head dimensions 104 to 120 take each step.
 // A key tile's steps are 32 queries (of a grid from the sequence's first) of one head each, from the LAST queries backwards, the group's heads
 // inside: every key tile of a sequence starts with the same step.
 // The steps of all tiles lie one behind the other on one axis, each tile's with OPERANDS units more for its operands and results, and every block takes an
 // equal share of that axis (share > 0): causal or ragged tiles have anything between one step and thousands, and in pieces of equal length left CUs
 // idle for a quarter of the time (six causal sequences of up to 5000 rows, 16 / 4 heads of 128: 796 + 16 us to meet, in shares 632 + 26, 0.99
-// PFLOP/s; where every block has as many steps in any case 1.1 PFLOP/s).  A tile that lies in several shares leaves a float sum in each, two places a block, which meet in
+// PFLOP/s counting all four products; where every block has as many steps in any case 1.1; matrix units busy 46 % of the clocks at 2.07 GHz).  A tile that lies in several shares leaves a float sum in each, two places a block, which meet in
 // packed_meet_kernel in order.  share 0: a block a tile.
 // =====================================================================================================================
 __device__ inline int steps_of(const PackedArgs& a, const Seq& e, int tile) {

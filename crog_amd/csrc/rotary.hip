@@ -5,8 +5,10 @@
 //
 // Angles.  A far position turns a fast pair thousands of times, so the product is formed in 64 bits, in revolutions; what is left of it after
 // the whole turns (|x| <= 1/2) is rounded once to 32 bits (2^-25 of a half turn) before the sine and cosine.
-// Bound: memory, each element read and written once (16384 rows of 16 + 4 heads x 128, bf16, 168 MB: 33.5 us, 5.0 TB/s, what a large copy reaches).  A block takes TOK rows and computes their pairs' sines and cosines ONCE, into LDS, for
-// all query and key heads of the row (40 heads x 64 pairs share 64 angles).
+// Bound: memory, each element read and written once (16384 rows of 16 + 4 heads x 128, bf16, 168 MB: 33.2 us, 5.0 TB/s, what a large copy reaches).  A
+// block takes TOK rows and computes their pairs' sines and cosines ONCE, into LDS, for all query and key heads of the row (40 heads x 64 pairs share 64
+// angles).  Not at that rate: columns behind the pairs, which are copied element by element, and calls whose pairs are no whole vectors (20 pairs of a head
+// of 80, bf16) or whose heads are not aligned, which go element by element throughout.
 #include "common.h"
 
 namespace {

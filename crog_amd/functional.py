@@ -1308,7 +1308,9 @@ def packed_attention(q, k, v, rows, scale=None):
     group, causal); any strides with adjacent columns (others are copied).  -> [rows, heads, dim].  scale: dim ** -0.5 by default.  dim is a
     multiple of 8 up to 128 (float32: of 4).  Rows behind the last sequence give zeros and get zero gradients, whatever they hold.  The same
     inputs give the same bits (no atomics).  A key or value that is not finite may reach every query of its own sequence, and no other; in the
-    backward pass that holds for any row.  Make the plan outside a captured graph."""
+    backward pass that holds for any row.  Scores, sums and the softmax are float32; bfloat16 inputs: the probabilities, and in the backward pass dS, are
+    rounded to bfloat16 for the matrix unit (summed over many keys, o and the gradients are off by up to 1.45 times their own rounding).  Make the plan
+    outside a captured graph and keep it as long as the graph."""
     qs, ks, dt, group = q.shape, k.shape, q.dtype, rows.group
     # (one condition for the calls that are right; what is wrong with another is found out behind it)
     if not (len(qs) == 3 == len(ks) and ks == v.shape and k.dtype == dt == v.dtype and qs[2] == ks[2] and qs[1] == ks[1] * group and ks[1] > 0
@@ -1367,7 +1369,8 @@ class RotaryFn(Function):
 
 def rotary(q, k, positions, axes):
     """Turns q [rows, heads, dim] and k [rows, key heads, dim] (k may be None) by their rows' positions, an int32 / int64 tensor [rows, axes]
-    ([rows] for one axis), as `axes` (packed.RotaryAxes) says; -> (q', k').  Columns behind the plan's pairs are copied."""
+    ([rows] for one axis), as `axes` (packed.RotaryAxes) says; -> (q', k').  Columns behind the plan's pairs are copied.  Keep the plan as long as
+    a graph captured with it."""
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
         raise ValueError(f"rotary: q and k must be [rows, heads, dim] with the same rows and dim, got {tuple(q.shape)}, {None if k is None else tuple(k.shape)}")
     if q.shape[0] > MAX_ROWS:
@@ -1438,7 +1441,8 @@ def gated_norm(x, y, *, post=None, gate: Optional[WRef] = None, pre=None, res_sc
     (1 without it).  rms: root-mean-square norms (no biases) instead of LayerNorm.  x, y: row matrices [..., C] of one shape and dtype, C up to
     8192; the second norm reads the float32 sum, u and h are rounded once.  The weights' gradients are added into the flat store in a fixed
     order (same bits every time).  One weight may stand in several places, of one call or of several, on whatever streams; only under
-    DistributedDataParallel a parameter belongs to one call a pass (the first that has added onto it announces it to its bucket)."""
+    DistributedDataParallel a parameter belongs to one call a pass (the first that has added onto it announces it to its bucket).  They are added
+    onto what the store holds: ParamStore.zero_grad clears it."""
     K.dcode(x)
     if x.shape != y.shape or x.dtype != y.dtype or x.dim() < 1:
         raise ValueError(f"gated_norm: x and y must have one shape and dtype, got {tuple(x.shape)} {x.dtype} and {tuple(y.shape)} {y.dtype}")

@@ -3,6 +3,8 @@ crog_amd.functional.packed_attention / rotary.
 
 A packed tensor holds the rows of all sequences of a batch one behind the other, [rows, heads, dim], with no padding between them: captions of
 different lengths, images of different sizes, documents.  Nothing here launches a kernel; a plan is two or three small tables on the device.
+A plan is made outside a captured graph, and outlives every graph that was captured with it (its replays read the tables; eager launches keep them
+themselves until they are through).
 """
 from __future__ import annotations
 
@@ -63,7 +65,7 @@ class PackedRows:
     lengths: query rows of each sequence; key_lengths: its key rows where they are others (cross-attention, or new tokens over what a
     sequence has behind it), by default the same rows.  group: query heads per key head.  causal: query i of a sequence with Lq queries and
     Lk keys sees keys j <= i + Lk - Lq, i.e. the last query sees them all; a query that sees none gets zeros.  A length may be zero.
-    device: where the tensors will live.  One plan serves every layer of a batch."""
+    device: where the tensors will live.  One plan serves every layer of a batch; it has to outlive the graphs captured with it."""
 
     def __init__(self, lengths: Sequence[int], key_lengths: Optional[Sequence[int]] = None, *, group: int = 1, causal: bool = False, device="cuda"):
         lq = _lengths("lengths", lengths)
@@ -114,7 +116,9 @@ class PackedRows:
 
     def splits(self, kv_heads: int, size: int):
         """(pieces, keys of a piece) of the forward and dQ passes' key axis; size: bytes of an element.  A single query over 8192 keys of 8 heads
-        would be 8 blocks on 256 CUs; in pieces of 256 keys it is 256.  Enough blocks, or short keys: one piece, no second launch."""
+        would be 8 blocks on 256 CUs; in pieces of 256 keys it is 256.  Enough blocks, or short keys: one piece, no second launch.  All
+        sequences are cut by the longest one's keys, and a tile counts as a block whatever its keys: one long sequence among many short ones is
+        walked by its own blocks alone."""
         blocks = max(self.n_row_tiles * kv_heads, 1)
         n = min(-(-FILL_BLOCKS // blocks), self.max_k // SPLIT_MIN[size])
         if n <= 1:
@@ -141,7 +145,7 @@ class RotaryAxes:
 
     pairs: how many pairs turn with each axis of the positions - (32,) for text, (16, 24, 24) for time, height and width.  Pair i of an axis
     with n pairs turns by position * theta^(-i / n).  interleaved: a pair is two neighbouring columns (2 i, 2 i + 1); otherwise column i and
-    column sum(pairs) + i.  One plan serves a model."""
+    column sum(pairs) + i.  One plan serves a model; it has to outlive the graphs captured with it."""
 
     def __init__(self, pairs: Sequence[int], *, theta: float = 10000.0, interleaved: bool = False, device="cuda"):
         sizes = [operator.index(n) for n in pairs]

@@ -624,6 +624,8 @@ int crog_preprocess_u8(const uint8_t* img, const uint8_t* masks, int B, int H, i
  * behind the other's, and each block walks `share` of them; a tile in several shares meets in a second launch.  0: a block a tile.
  * partial: the larger of 2 * ceil(total_units * kv_heads / share) * 128 * 2 * head_dim floats and, for the splits of dQ,
  * splits * kv_heads * group * rows_q * head_dim.
+ * scale * log2(e) has to be a finite float.  A table that holds something else than this gives wrong results, but no access outside the tensors, lse, D
+ * and partial.  Tables and workspace have to outlive a graph captured with them.
  * Rows outside every sequence are not read and not written.  Non-finite values of a key or value row may reach every query row of its own
  * sequence (also through a probability of zero), never another sequence; in the backward those of any row reach its sequence. */
 int crog_packed_attn_fwd(int dtype, const void* Q, int64_t ldq, int64_t hsq, const void* K, int64_t ldk, int64_t hsk,
