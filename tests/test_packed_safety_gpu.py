@@ -131,7 +131,9 @@ def test_gated_norms_on_several_streams_share_weights(mode):
             assert all(torch.equal(a, b) for a, b in zip(run(where), want))
 
 
-def test_gated_norm_beside_the_frameworks_layers_captured_and_replayed():
+@pytest.mark.parametrize("warm", ["side", "main", "both"])
+def test_gated_norm_beside_the_frameworks_layers_captured_and_replayed(warm):
+    from crog_amd import functional as Fn
     m, st, r = store_of(**WEIGHTS)
     x, y, gu, gh = (dev(T, C, seed=i) for i in (1, 2, 3, 4))
     x.requires_grad_(), y.requires_grad_()
@@ -140,10 +142,14 @@ def test_gated_norm_beside_the_frameworks_layers_captured_and_replayed():
         outs = block(r, x, y)
         return (*outs, *torch.autograd.grad(outs, (x, y), (gu, gh)))
     side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):
+    if warm != "main":
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+    if warm != "side":      # (the last gradients before the capture were added on the device's own stream)
         step()
-    torch.cuda.current_stream().wait_stream(side)
+        torch.autograd.grad(Fn.gated_norm(x, y, gate=r["gate"])[0], x, gu)
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         outs = step()
@@ -329,3 +335,45 @@ def test_dq_of_few_rows_carries_the_rests(n, group):
             edd = edd + (gg.abs() * ep * (p @ vv.abs())).sum(1, keepdim=True) * (n <= 64)
             eds = p / 8 * (edd + U * (D + 4) * (gg.abs() @ vv.abs().T)) + ds.abs() * (h * h + ep + 4 * U)
             within(dq[at, g], want, h * want.abs() + (eds @ kk.abs() + U * n * (ds.abs() @ kk.abs())) * (1 + h), f"dq of sequence {s}")
+
+
+def test_gated_norm_captured_on_streams_of_its_own():
+    """Two gated norms with one weight, captured alone (nothing else forks) and on two streams of the capture, after eager passes on the device's own stream."""
+    from crog_amd import functional as Fn
+    m, st, r = store_of(**WEIGHTS)
+    x, y, gu, gh = (dev(T, C, dtype=torch.bfloat16, seed=i) for i in (1, 2, 3, 4))
+    x.requires_grad_(), y.requires_grad_()
+
+    def one():
+        return Fn.gated_norm(x, y, post=(r["post_w"], r["post_b"]), gate=r["gate"], pre=(r["norm_w"], r["norm_b"]))
+
+    def alone():
+        return torch.autograd.grad(one(), (x, y), (gu, gh))
+
+    def forked():
+        here, other = torch.cuda.current_stream(), streams[0]
+        other.wait_stream(here)
+        with torch.cuda.stream(other):
+            outs = one()
+        outs = one() + outs
+        here.wait_stream(other)
+        return torch.autograd.grad(outs, (x, y), (gu, gh, gu, gh))
+    streams = [torch.cuda.Stream()]
+    for step in (alone, forked):
+        step()
+        alone()
+        st.zero_grad()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step()
+        for turn in range(3):
+            with torch.no_grad():
+                for i, t in enumerate((x, y, gu, gh)):
+                    t.copy_(dev(T, C, dtype=torch.bfloat16, seed=10 * turn + i))
+            st.zero_grad()
+            want = step()
+            once = st.G.clone()
+            st.zero_grad()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)) and torch.equal(st.G, once), (step.__name__, turn)
